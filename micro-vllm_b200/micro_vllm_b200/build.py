@@ -1,11 +1,14 @@
-"""Build libmvdecode.so in-tree for sm_100a with nvcc.
+"""Build libmvdecode.so and libmvquant.so in-tree for sm_100a with nvcc.
 
     python -m micro_vllm_b200.build        (from the micro-vllm_b200/ source root)
 
-The library links the CUDA runtime statically and resolves the driver's
-tensor-map encoder at run time, so it needs only the NVIDIA driver next to it.
+libmvdecode.so holds the decode path (include/mvdecode.h), libmvquant.so the
+operators with 4-bit weights and 8-bit rows (include/mvquant.h). Both link the
+CUDA runtime statically and the first resolves the driver's tensor-map encoder
+at run time, so they need only the NVIDIA driver next to them.
 """
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -15,6 +18,7 @@ PACKAGE_DIR = Path(__file__).resolve().parent
 CSRC_DIR = PACKAGE_DIR / 'csrc'
 LIB_DIR = PACKAGE_DIR / 'lib'
 LIB_PATH = LIB_DIR / 'libmvdecode.so'
+QUANT_LIB_PATH = LIB_DIR / 'libmvquant.so'
 INCLUDE_DIR = PACKAGE_DIR.parents[1] / 'include'
 
 NVCC_FLAGS = [
@@ -37,27 +41,54 @@ def sources():
     return sorted(CSRC_DIR.glob('*.cu')) + sorted(CSRC_DIR.glob('*.cuh'))
 
 
-def is_stale() -> bool:
-    if not LIB_PATH.exists():
+# Library -> the one translation unit it is made of and the header it implements.
+LIBRARIES = {
+    LIB_PATH: (CSRC_DIR / 'mv_capi.cu', INCLUDE_DIR / 'mvdecode.h'),
+    QUANT_LIB_PATH: (CSRC_DIR / 'mvq_capi.cu', INCLUDE_DIR / 'mvquant.h'),
+}
+
+
+def _reached(path: Path, seen=None):
+    """``path`` and the files of csrc/ that it includes."""
+    seen = set() if seen is None else seen
+    if path not in seen:
+        seen.add(path)
+        for name in re.findall(r'^#include "([^"]+)"', path.read_text(), flags=re.MULTILINE):
+            if (CSRC_DIR / name).exists():
+                _reached(CSRC_DIR / name, seen)
+    return seen
+
+
+def _library_is_stale(library: Path) -> bool:
+    if not library.exists():
         return True
-    built = LIB_PATH.stat().st_mtime
-    inputs = list(sources()) + [INCLUDE_DIR / 'mvdecode.h', Path(__file__)]
-    return any(path.stat().st_mtime > built for path in inputs)
+    unit, header = LIBRARIES[library]
+    built = library.stat().st_mtime
+    return any(path.stat().st_mtime > built for path in [*_reached(unit), header, Path(__file__)])
+
+
+def is_stale() -> bool:
+    return any(_library_is_stale(library) for library in LIBRARIES)
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile the library unless it is newer than every source; return its path."""
-    if not force and not is_stale():
-        return LIB_PATH
+    """Compile each library unless it is newer than every source; return the decode library's path."""
     LIB_DIR.mkdir(parents=True, exist_ok=True)
-    tmp = LIB_PATH.with_suffix('.so.tmp')
-    cmd = [nvcc_path(), *NVCC_FLAGS, '-I', str(INCLUDE_DIR), '-o', str(tmp),
-           str(CSRC_DIR / 'mv_capi.cu')]
-    if verbose:
-        cmd.insert(1, '-Xptxas=-v')
-        print(' '.join(cmd), file=sys.stderr)
-    subprocess.run(cmd, check=True)
-    os.replace(tmp, LIB_PATH)
+    running = []
+    for library, (unit, _) in LIBRARIES.items():
+        if not force and not _library_is_stale(library):
+            continue
+        tmp = library.with_suffix('.so.tmp')
+        cmd = [nvcc_path(), *NVCC_FLAGS, '-I', str(INCLUDE_DIR), '-o', str(tmp), str(unit)]
+        if verbose:
+            cmd.insert(1, '-Xptxas=-v')
+            print(' '.join(cmd), file=sys.stderr)
+        running.append((library, tmp, cmd, subprocess.Popen(cmd)))
+    codes = [process.wait() for *_, process in running]
+    for (library, tmp, cmd, _), code in zip(running, codes):
+        if code:
+            raise subprocess.CalledProcessError(code, cmd)
+        os.replace(tmp, library)
     return LIB_PATH
 
 

@@ -1,0 +1,392 @@
+// C ABI of libmvquant.so (include/mvquant.h): argument checks, kernel choice, launches.
+#include "mvquant.h"
+
+#include <cmath>
+#include <cstdarg>
+#include <cstdio>
+#include <mutex>
+
+#include "quant_rows.cuh"
+#include "w4_linear.cuh"
+
+namespace {
+
+thread_local char g_error[512];
+
+int fail(int code, const char* fmt, ...) {
+    va_list args;
+    va_start(args, fmt);
+    vsnprintf(g_error, sizeof(g_error), fmt, args);
+    va_end(args);
+    return code;
+}
+
+int cuda_fail(cudaError_t err, const char* what) {
+    return fail(MVQ_ERR_CUDA, "%s: %s", what, cudaGetErrorString(err));
+}
+
+constexpr int kMaxDevices = 64;
+
+// Streaming multiprocessors of the current device (asked once per device).
+int device_sms(int* device, int* sms) {
+    static std::mutex mutex;
+    static int known[kMaxDevices];
+    cudaError_t err = cudaGetDevice(device);
+    if (err != cudaSuccess) return cuda_fail(err, "cudaGetDevice");
+    if (*device < 0 || *device >= kMaxDevices) return fail(MVQ_ERR_UNSUPPORTED, "device index %d out of range", *device);
+    std::lock_guard<std::mutex> lock(mutex);
+    if (known[*device] == 0) {
+        int n = 0;
+        err = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, *device);
+        if (err != cudaSuccess) return cuda_fail(err, "cudaDeviceGetAttribute");
+        known[*device] = n;
+    }
+    *sms = known[*device];
+    return MVQ_OK;
+}
+
+bool float_dtype(int64_t d) { return d == MVQ_DTYPE_F32 || d == MVQ_DTYPE_F16 || d == MVQ_DTYPE_BF16; }
+int64_t dtype_size(int64_t d) { return d == MVQ_DTYPE_F32 ? 4 : d == MVQ_DTYPE_F16 || d == MVQ_DTYPE_BF16 ? 2 : 1; }
+uintptr_t address(const void* p) { return reinterpret_cast<uintptr_t>(p); }
+
+// Programmatic stream serialization (the kernels wait before they read), and a
+// cluster along x where one is asked for.
+template <typename... Params, typename... Args>
+cudaError_t launch(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, int cluster, void* stream,
+                   Args&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = static_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+
+// ------------------------------------------------------------------- weights
+
+constexpr int64_t kMaxSize = int64_t(1) << 30;
+
+int check_weight(const void* records, int64_t n, int64_t k, int64_t group, int64_t scale_dtype) {
+    if (!records) return fail(MVQ_ERR_INVALID_ARGUMENT, "records must not be NULL");
+    if (address(records) % 16) return fail(MVQ_ERR_INVALID_ARGUMENT, "records must be 16-byte aligned");
+    if (n <= 0 || k <= 0) return fail(MVQ_ERR_INVALID_ARGUMENT, "sizes must be positive");
+    if (n > kMaxSize || k > kMaxSize) return fail(MVQ_ERR_UNSUPPORTED, "sizes must be at most 2^30");
+    if (group != 32 && group != 64 && group != 128)
+        return fail(MVQ_ERR_UNSUPPORTED, "group must be 32, 64 or 128");
+    if (scale_dtype != MVQ_DTYPE_F16 && scale_dtype != MVQ_DTYPE_BF16)
+        return fail(MVQ_ERR_INVALID_ARGUMENT, "scale_dtype must be MVQ_DTYPE_F16 or MVQ_DTYPE_BF16");
+    return MVQ_OK;
+}
+
+int record_bytes(int64_t group, int64_t has_zeros) {
+    return mvq::kCodeBytes + static_cast<int>(mvq::kChunk / group) * (has_zeros ? 192 : 128);
+}
+
+template <int XT, int NB, int GROUP>
+int launch_linear(const mvq::LinearParams& p, int device, int tiles, int blocks, void* stream) {
+    auto kernel = mvq::w4_linear_kernel<XT, NB, GROUP>;
+    constexpr int kMost = mvq::kWarps * mvq::kStages * (mvq::kCodeBytes + mvq::kChunk / GROUP * 192);
+    static std::mutex mutex;
+    static bool ready[kMaxDevices];
+    {
+        std::lock_guard<std::mutex> lock(mutex);
+        if (!ready[device]) {
+            cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
+            if (err == cudaSuccess)
+                err = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                           static_cast<int>(cudaSharedmemCarveoutMaxShared));
+            if (err != cudaSuccess) return cuda_fail(err, "cudaFuncSetAttribute");
+            ready[device] = true;
+        }
+    }
+    const size_t smem = static_cast<size_t>(mvq::kWarps) * mvq::kStages * p.record_bytes;
+    const dim3 grid(static_cast<unsigned>(tiles) * p.cluster, blocks);
+    const cudaError_t err = launch(kernel, grid, mvq::kThreads, smem, p.cluster, stream, p);
+    return err == cudaSuccess ? MVQ_OK : cuda_fail(err, "4-bit linear kernel launch");
+}
+
+template <int XT, int NB>
+int launch_linear_group(const mvq::LinearParams& p, int64_t group, int device, int tiles, int blocks, void* stream) {
+    switch (group) {
+        case 32: return launch_linear<XT, NB, 32>(p, device, tiles, blocks, stream);
+        case 64: return launch_linear<XT, NB, 64>(p, device, tiles, blocks, stream);
+        default: return launch_linear<XT, NB, 128>(p, device, tiles, blocks, stream);
+    }
+}
+
+template <int XT>
+int launch_linear_tokens(const mvq::LinearParams& p, int64_t group, int device, int sms, int tiles, void* stream) {
+    // Tokens per pass over the records: 8, 16 or 32 (fp32 x is three numbers per element: 8).
+    const int most = XT == mvq::kF32 ? 1 : 4;
+    int nb = p.m <= 8 ? 1 : p.m <= 16 ? 2 : 4;
+    if (nb > most) nb = most;
+    const int64_t blocks = (static_cast<int64_t>(p.m) + 8 * nb - 1) / (8 * nb);
+    if (blocks > 65535) return fail(MVQ_ERR_UNSUPPORTED, "too many rows of x for one call");
+    mvq::LinearParams q = p;
+    q.cluster = 1;
+    while (q.cluster < 8 && static_cast<int64_t>(tiles) * blocks * q.cluster < 3 * static_cast<int64_t>(sms) &&
+           p.chunks > mvq::kWarps * q.cluster)
+        q.cluster *= 2;
+    if (static_cast<int64_t>(tiles) * q.cluster >= (int64_t(1) << 31))
+        return fail(MVQ_ERR_UNSUPPORTED, "too many weight rows for one call");
+    const int b = static_cast<int>(blocks);
+    if constexpr (XT != mvq::kF32) {
+        if (nb == 4) return launch_linear_group<XT, 4>(q, group, device, tiles, b, stream);
+        if (nb == 2) return launch_linear_group<XT, 2>(q, group, device, tiles, b, stream);
+    }
+    return launch_linear_group<XT, 1>(q, group, device, tiles, b, stream);
+}
+
+// ---------------------------------------------------------------------- rows
+
+// Threads and runs of eight per thread for rows of `width` elements.
+struct RowShape {
+    int threads;
+    int held;  // runs of eight elements a thread holds: 1, 2, 4 or 8; 0: none, the row is read twice
+};
+
+// `most`: the most runs that a thread may hold.
+RowShape row_shape(int64_t width, int64_t rows, int sms, int most) {
+    const int64_t runs = (width + 7) / 8;
+    // Few rows: a thread per run, which spreads the row's latency over the CTA.
+    // Many rows: two runs a thread.
+    int held = rows > 2 * static_cast<int64_t>(sms) ? 2 : 1;
+    while (held <= most && runs > static_cast<int64_t>(held) * mvq::max_row_threads(held)) held *= 2;
+    if (held > most) return {mvq::max_row_threads(0), 0};
+    return {static_cast<int>(((runs + held - 1) / held + 31) / 32 * 32), held};
+}
+
+template <typename T, int OUT, bool RUNS, template <typename, int, bool, int> class Kernel, typename P>
+cudaError_t launch_row_held(const P& p, RowShape shape, int64_t rows, void* stream) {
+    const dim3 grid(static_cast<unsigned>(rows));
+    switch (shape.held) {
+        case 1: return launch(Kernel<T, OUT, RUNS, 1>::get(), grid, shape.threads, 0, 1, stream, p);
+        case 2: return launch(Kernel<T, OUT, RUNS, 2>::get(), grid, shape.threads, 0, 1, stream, p);
+        default: break;
+    }
+    if constexpr (RUNS) {
+        if (shape.held == 4) return launch(Kernel<T, OUT, RUNS, 4>::get(), grid, shape.threads, 0, 1, stream, p);
+        if (shape.held == 8) return launch(Kernel<T, OUT, RUNS, 8>::get(), grid, shape.threads, 0, 1, stream, p);
+    }
+    return launch(Kernel<T, OUT, RUNS, 0>::get(), grid, shape.threads, 0, 1, stream, p);
+}
+
+template <typename T, int OUT, template <typename, int, bool, int> class Kernel, typename P>
+cudaError_t launch_row_access(const P& p, bool runs, int64_t width, int64_t rows, int sms, void* stream) {
+    const RowShape shape = row_shape(width, rows, sms, runs ? 8 : 2);
+    return runs ? launch_row_held<T, OUT, true, Kernel>(p, shape, rows, stream)
+                : launch_row_held<T, OUT, false, Kernel>(p, shape, rows, stream);
+}
+
+template <int OUT, template <typename, int, bool, int> class Kernel, typename P>
+cudaError_t launch_row_type(const P& p, int64_t dtype, bool runs, int64_t width, int64_t rows, int sms, void* stream) {
+    if (dtype == MVQ_DTYPE_F32) return launch_row_access<float, OUT, Kernel>(p, runs, width, rows, sms, stream);
+    if (dtype == MVQ_DTYPE_F16) return launch_row_access<__half, OUT, Kernel>(p, runs, width, rows, sms, stream);
+    return launch_row_access<__nv_bfloat16, OUT, Kernel>(p, runs, width, rows, sms, stream);
+}
+
+template <typename T, int OUT, bool RUNS, int C>
+struct NormKernel {
+    static auto get() { return mvq::add_rms_norm_kernel<T, OUT, RUNS, C>; }
+};
+template <typename T, int OUT, bool RUNS, int C>
+struct SiluKernel {
+    static auto get() { return mvq::silu_mul_quant_kernel<T, OUT, RUNS, C>; }
+};
+
+int check_rows(int64_t rows, int64_t width, int64_t dtype) {
+    if (rows <= 0 || width <= 0) return fail(MVQ_ERR_INVALID_ARGUMENT, "sizes must be positive");
+    if (rows >= (int64_t(1) << 31) || width > kMaxSize)
+        return fail(MVQ_ERR_UNSUPPORTED, "rows must be below 2^31 and at most 2^30 elements wide");
+    if (!float_dtype(dtype))
+        return fail(MVQ_ERR_INVALID_ARGUMENT, "dtype must be MVQ_DTYPE_F32, MVQ_DTYPE_F16 or MVQ_DTYPE_BF16");
+    return MVQ_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int mvq_abi_version(void) { return MVQ_ABI_VERSION; }
+
+const char* mvq_last_error(void) { return g_error; }
+
+int mvq_w4_linear(const MvqLinearArgs* a, void* stream) try {
+    if (!a) return fail(MVQ_ERR_INVALID_ARGUMENT, "args must not be NULL");
+    int rc = check_weight(a->records, a->n, a->k, a->group, a->scale_dtype);
+    if (rc != MVQ_OK) return rc;
+    if (!a->x || !a->out) return fail(MVQ_ERR_INVALID_ARGUMENT, "x and out must not be NULL");
+    if (a->m <= 0) return fail(MVQ_ERR_INVALID_ARGUMENT, "sizes must be positive");
+    if (a->m > kMaxSize) return fail(MVQ_ERR_UNSUPPORTED, "sizes must be at most 2^30");
+    if (a->x_dtype < 0 || a->x_dtype > MVQ_DTYPE_E4M3)
+        return fail(MVQ_ERR_INVALID_ARGUMENT, "x_dtype must be an MVQ_DTYPE_* value");
+    if (!float_dtype(a->out_dtype))
+        return fail(MVQ_ERR_INVALID_ARGUMENT, "out_dtype must be MVQ_DTYPE_F32, MVQ_DTYPE_F16 or MVQ_DTYPE_BF16");
+    if (a->m > 1 && (a->x_stride_row < 0 || a->out_stride_row < a->n || (a->residual && a->residual_stride_row < 0)))
+        return fail(MVQ_ERR_INVALID_ARGUMENT, "row strides must be nonnegative and out's rows must not overlap");
+    int device, sms;
+    rc = device_sms(&device, &sms);
+    if (rc != MVQ_OK) return rc;
+    const int64_t size = dtype_size(a->x_dtype);
+    const int64_t run = size == 1 ? 8 : 16;  // bytes of a vector load of x
+    mvq::LinearParams p = {};
+    p.x = a->x;
+    p.x_stride = a->x_stride_row;
+    p.x_scale = static_cast<const float*>(a->x_scale);
+    p.records = static_cast<const uint8_t*>(a->records);
+    p.n = static_cast<int>(a->n);
+    p.k = static_cast<int>(a->k);
+    p.m = static_cast<int>(a->m);
+    p.chunks = static_cast<int>((a->k + mvq::kChunk - 1) / mvq::kChunk);
+    p.record_bytes = record_bytes(a->group, a->has_zeros);
+    p.has_zeros = a->has_zeros != 0;
+    p.scale_bf16 = a->scale_dtype == MVQ_DTYPE_BF16;
+    p.x_runs = a->k % 8 == 0 && address(a->x) % run == 0 && (a->m == 1 || a->x_stride_row * size % run == 0);
+    p.bias = a->bias;
+    p.residual = a->residual;
+    p.residual_stride = a->residual_stride_row;
+    p.out = a->out;
+    p.out_stride = a->out_stride_row;
+    p.out_dtype = static_cast<int>(a->out_dtype);
+    const int tiles = static_cast<int>((a->n + mvq::kTileRows - 1) / mvq::kTileRows);
+    switch (a->x_dtype) {
+        case MVQ_DTYPE_F32: return launch_linear_tokens<mvq::kF32>(p, a->group, device, sms, tiles, stream);
+        case MVQ_DTYPE_F16: return launch_linear_tokens<mvq::kF16>(p, a->group, device, sms, tiles, stream);
+        case MVQ_DTYPE_BF16: return launch_linear_tokens<mvq::kBF16>(p, a->group, device, sms, tiles, stream);
+        case MVQ_DTYPE_I8: return launch_linear_tokens<mvq::kI8>(p, a->group, device, sms, tiles, stream);
+        default: return launch_linear_tokens<mvq::kE4M3>(p, a->group, device, sms, tiles, stream);
+    }
+} catch (...) {
+    return fail(MVQ_ERR_CUDA, "unexpected C++ exception");
+}
+
+int mvq_w4_dequantize(const MvqDequantizeArgs* a, void* stream) try {
+    if (!a) return fail(MVQ_ERR_INVALID_ARGUMENT, "args must not be NULL");
+    int rc = check_weight(a->records, a->n, a->k, a->group, a->scale_dtype);
+    if (rc != MVQ_OK) return rc;
+    if (!a->out) return fail(MVQ_ERR_INVALID_ARGUMENT, "out must not be NULL");
+    if (!float_dtype(a->out_dtype))
+        return fail(MVQ_ERR_INVALID_ARGUMENT, "out_dtype must be MVQ_DTYPE_F32, MVQ_DTYPE_F16 or MVQ_DTYPE_BF16");
+    if (a->n > 1 && a->out_stride_row < a->k)
+        return fail(MVQ_ERR_INVALID_ARGUMENT, "out's rows must not overlap");
+    const int chunks = static_cast<int>((a->k + mvq::kChunk - 1) / mvq::kChunk);
+    const int64_t total = (a->n + mvq::kTileRows - 1) / mvq::kTileRows * chunks;
+    if (total >= (int64_t(1) << 33)) return fail(MVQ_ERR_UNSUPPORTED, "the weight is too large for one call");
+    const int64_t size = dtype_size(a->out_dtype);
+    const int runs = address(a->out) % 16 == 0 && (a->n == 1 || a->out_stride_row * size % 16 == 0);
+    const dim3 grid(static_cast<unsigned>((total + 7) / 8));
+    const int bytes = record_bytes(a->group, a->has_zeros), bf16 = a->scale_dtype == MVQ_DTYPE_BF16;
+    const uint8_t* records = static_cast<const uint8_t*>(a->records);
+    const int group = static_cast<int>(a->group), zeros = a->has_zeros != 0;
+    const int n = static_cast<int>(a->n), k = static_cast<int>(a->k);
+    cudaError_t err;
+    if (a->out_dtype == MVQ_DTYPE_F32)
+        err = launch(mvq::w4_dequantize_kernel<float>, grid, 256, 0, 1, stream, records, total, chunks, bytes, group,
+                     zeros, bf16, n, k, static_cast<float*>(a->out), a->out_stride_row, runs);
+    else if (a->out_dtype == MVQ_DTYPE_F16)
+        err = launch(mvq::w4_dequantize_kernel<__half>, grid, 256, 0, 1, stream, records, total, chunks, bytes, group,
+                     zeros, bf16, n, k, static_cast<__half*>(a->out), a->out_stride_row, runs);
+    else
+        err = launch(mvq::w4_dequantize_kernel<__nv_bfloat16>, grid, 256, 0, 1, stream, records, total, chunks, bytes,
+                     group, zeros, bf16, n, k, static_cast<__nv_bfloat16*>(a->out), a->out_stride_row, runs);
+    return err == cudaSuccess ? MVQ_OK : cuda_fail(err, "4-bit dequantize kernel launch");
+} catch (...) {
+    return fail(MVQ_ERR_CUDA, "unexpected C++ exception");
+}
+
+int mvq_add_rms_norm(const MvqNormArgs* a, void* stream) try {
+    if (!a) return fail(MVQ_ERR_INVALID_ARGUMENT, "args must not be NULL");
+    int rc = check_rows(a->rows, a->hidden, a->dtype);
+    if (rc != MVQ_OK) return rc;
+    if (!a->x || !a->weight || !a->out) return fail(MVQ_ERR_INVALID_ARGUMENT, "x, weight and out must not be NULL");
+    const bool eight = a->out_dtype == MVQ_DTYPE_I8 || a->out_dtype == MVQ_DTYPE_E4M3;
+    if (!eight && a->out_dtype != a->dtype)
+        return fail(MVQ_ERR_INVALID_ARGUMENT, "out_dtype must be dtype, MVQ_DTYPE_I8 or MVQ_DTYPE_E4M3");
+    if (eight != (a->scales != nullptr))
+        return fail(MVQ_ERR_INVALID_ARGUMENT, "8-bit outputs, and only those, come with scales");
+    if (!(a->eps >= 0.0) || std::isinf(a->eps))
+        return fail(MVQ_ERR_INVALID_ARGUMENT, "eps must be finite and nonnegative");
+    if (a->rows > 1 && (a->x_stride_row < 0 || (a->residual && a->residual_stride_row < 0) ||
+                        a->out_stride_row < a->hidden ||
+                        (a->residual_out && a->residual_out_stride_row < a->hidden)))
+        return fail(MVQ_ERR_INVALID_ARGUMENT, "row strides must be nonnegative and outputs' rows must not overlap");
+    int device, sms;
+    rc = device_sms(&device, &sms);
+    if (rc != MVQ_OK) return rc;
+    const int64_t size = dtype_size(a->dtype);
+    const bool one = a->rows == 1;  // strides that no row uses
+    const uintptr_t wide = address(a->x) | address(a->residual) | address(a->weight) | address(a->residual_out) |
+                           (one ? 0 : static_cast<uintptr_t>(a->x_stride_row * size) |
+                                          (a->residual ? static_cast<uintptr_t>(a->residual_stride_row * size) : 0) |
+                                          (a->residual_out ? static_cast<uintptr_t>(a->residual_out_stride_row * size) : 0));
+    const int64_t out_run = eight ? 8 : 16;
+    const bool runs = a->hidden % 8 == 0 && wide % 16 == 0 && address(a->out) % out_run == 0 &&
+                      (one || a->out_stride_row * (eight ? 1 : size) % out_run == 0);
+    mvq::NormParams p = {};
+    p.x = a->x;
+    p.x_stride = a->x_stride_row;
+    p.residual = a->residual;
+    p.residual_stride = a->residual_stride_row;
+    p.weight = a->weight;
+    p.out = a->out;
+    p.out_stride = a->out_stride_row;
+    p.scales = static_cast<float*>(a->scales);
+    p.residual_out = a->residual_out;
+    p.residual_out_stride = a->residual_out_stride_row;
+    p.hidden = static_cast<int>(a->hidden);
+    p.eps = static_cast<float>(a->eps);
+    cudaError_t err;
+    if (a->out_dtype == MVQ_DTYPE_I8)
+        err = launch_row_type<mvq::kOutI8, NormKernel>(p, a->dtype, runs, a->hidden, a->rows, sms, stream);
+    else if (a->out_dtype == MVQ_DTYPE_E4M3)
+        err = launch_row_type<mvq::kOutE4M3, NormKernel>(p, a->dtype, runs, a->hidden, a->rows, sms, stream);
+    else
+        err = launch_row_type<mvq::kOutSame, NormKernel>(p, a->dtype, runs, a->hidden, a->rows, sms, stream);
+    return err == cudaSuccess ? MVQ_OK : cuda_fail(err, "add-RMSNorm kernel launch");
+} catch (...) {
+    return fail(MVQ_ERR_CUDA, "unexpected C++ exception");
+}
+
+int mvq_silu_mul_quant(const MvqSiluArgs* a, void* stream) try {
+    if (!a) return fail(MVQ_ERR_INVALID_ARGUMENT, "args must not be NULL");
+    int rc = check_rows(a->rows, a->width, a->dtype);
+    if (rc != MVQ_OK) return rc;
+    if (!a->gate_up || !a->out || !a->scales)
+        return fail(MVQ_ERR_INVALID_ARGUMENT, "gate_up, out and scales must not be NULL");
+    if (a->out_dtype != MVQ_DTYPE_I8 && a->out_dtype != MVQ_DTYPE_E4M3)
+        return fail(MVQ_ERR_INVALID_ARGUMENT, "out_dtype must be MVQ_DTYPE_I8 or MVQ_DTYPE_E4M3");
+    if (a->rows > 1 && (a->stride_row < 0 || a->out_stride_row < a->width))
+        return fail(MVQ_ERR_INVALID_ARGUMENT, "row strides must be nonnegative and out's rows must not overlap");
+    int device, sms;
+    rc = device_sms(&device, &sms);
+    if (rc != MVQ_OK) return rc;
+    const int64_t size = dtype_size(a->dtype);
+    const bool one = a->rows == 1;
+    const bool runs = a->width % 8 == 0 && address(a->gate_up) % 16 == 0 && address(a->out) % 8 == 0 &&
+                      (one || (a->stride_row * size % 16 == 0 && a->out_stride_row % 8 == 0));
+    mvq::SiluParams p = {};
+    p.gate_up = a->gate_up;
+    p.stride = a->stride_row;
+    p.out = a->out;
+    p.out_stride = a->out_stride_row;
+    p.scales = static_cast<float*>(a->scales);
+    p.width = static_cast<int>(a->width);
+    const cudaError_t err =
+        a->out_dtype == MVQ_DTYPE_I8
+            ? launch_row_type<mvq::kOutI8, SiluKernel>(p, a->dtype, runs, a->width, a->rows, sms, stream)
+            : launch_row_type<mvq::kOutE4M3, SiluKernel>(p, a->dtype, runs, a->width, a->rows, sms, stream);
+    return err == cudaSuccess ? MVQ_OK : cuda_fail(err, "SiLU-mul-quantize kernel launch");
+} catch (...) {
+    return fail(MVQ_ERR_CUDA, "unexpected C++ exception");
+}
+
+}  // extern "C"
