@@ -56,7 +56,7 @@ extern "C" {
  * (i * ceil(k / 128) + j) * record_bytes of `records` and holds
  *   4096 bytes of codes: [h 0..3][p 0..1][lane 0..31][word 0..3] 32-bit words.
  *     With g = lane / 4, t = lane % 4 and word = 2 q + e, the word holds the
- *     columns c = 32 h + 8 t + 4 e + s (s 0..3) of rows 32 p + 16 q + g (the low
+ *     columns c = 32 h + 16 e + 4 t + s (s 0..3) of rows 32 p + 16 q + g (the low
  *     nibbles of bytes) and 32 p + 16 q + 8 + g (the high nibbles), s = 0, 2, 1, 3
  *     in bytes 0..3, each nibble the code with its highest bit inverted;
  *   128 bytes of scales for each group of the chunk: [g 0..7][p][q][half], fp16
@@ -110,6 +110,15 @@ typedef struct MvqSiluArgs {
     int64_t rows; int64_t width; int64_t dtype; int64_t out_dtype;
 } MvqSiluArgs;
 MVQ_API int mvq_silu_mul_quant(const MvqSiluArgs* args, void* stream);
+
+/*
+ * Sticky bit of this library's kernels on `device`: 1 if a bounded wait gave up
+ * (its call's result is NaN). Reading synchronises with the device's legacy
+ * stream, as mv_device_status does for libmvdecode.so.
+ */
+#define MVQ_DEVICE_STATUS_WAIT_TIMEOUT 1
+MVQ_API int mvq_device_status(int32_t device, uint32_t* status);
+MVQ_API int mvq_clear_device_status(int32_t device);
 
 MVQ_API int mvq_abi_version(void);
 

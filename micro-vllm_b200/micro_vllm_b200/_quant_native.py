@@ -38,7 +38,9 @@ pack_norm = _packer(NORM_FIELDS)
 pack_silu = _packer(SILU_FIELDS)
 
 ENTRY_POINTS = ('mvq_w4_linear', 'mvq_w4_dequantize', 'mvq_add_rms_norm', 'mvq_silu_mul_quant')
-EXPORTED_SYMBOLS = ENTRY_POINTS + ('mvq_abi_version', 'mvq_last_error')
+EXPORTED_SYMBOLS = ENTRY_POINTS + ('mvq_abi_version', 'mvq_last_error', 'mvq_device_status',
+                                   'mvq_clear_device_status')
+DEVICE_STATUS_WAIT_TIMEOUT = 1
 
 
 @lru_cache(maxsize=1)
@@ -53,6 +55,9 @@ def library() -> ctypes.CDLL:
         fn = getattr(lib, name)
         fn.restype = ctypes.c_int
         fn.argtypes = [ctypes.c_char_p, ctypes.c_void_p]
+    lib.mvq_device_status.restype = lib.mvq_clear_device_status.restype = ctypes.c_int
+    lib.mvq_device_status.argtypes = [ctypes.c_int32, ctypes.POINTER(ctypes.c_uint32)]
+    lib.mvq_clear_device_status.argtypes = [ctypes.c_int32]
     lib.mvq_abi_version.restype = ctypes.c_int
     lib.mvq_last_error.restype = ctypes.c_char_p
     version = lib.mvq_abi_version()

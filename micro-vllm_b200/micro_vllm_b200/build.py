@@ -41,10 +41,11 @@ def sources():
     return sorted(CSRC_DIR.glob('*.cu')) + sorted(CSRC_DIR.glob('*.cuh'))
 
 
-# Library -> the one translation unit it is made of and the header it implements.
+# Library -> the translation units it is made of and the header it implements.
 LIBRARIES = {
-    LIB_PATH: (CSRC_DIR / 'mv_capi.cu', INCLUDE_DIR / 'mvdecode.h'),
-    QUANT_LIB_PATH: (CSRC_DIR / 'mvq_capi.cu', INCLUDE_DIR / 'mvquant.h'),
+    LIB_PATH: ([CSRC_DIR / 'mv_capi.cu'], INCLUDE_DIR / 'mvdecode.h'),
+    QUANT_LIB_PATH: ([CSRC_DIR / 'mvq_capi.cu', CSRC_DIR / 'w4_linear.cu', CSRC_DIR / 'w4_wide.cu'],
+                     INCLUDE_DIR / 'mvquant.h'),
 }
 
 
@@ -62,9 +63,10 @@ def _reached(path: Path, seen=None):
 def _library_is_stale(library: Path) -> bool:
     if not library.exists():
         return True
-    unit, header = LIBRARIES[library]
+    units, header = LIBRARIES[library]
     built = library.stat().st_mtime
-    return any(path.stat().st_mtime > built for path in [*_reached(unit), header, Path(__file__)])
+    inputs = set().union(*map(_reached, units)) | {header, Path(__file__)}
+    return any(path.stat().st_mtime > built for path in inputs)
 
 
 def is_stale() -> bool:
@@ -75,11 +77,12 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     """Compile each library unless it is newer than every source; return the decode library's path."""
     LIB_DIR.mkdir(parents=True, exist_ok=True)
     running = []
-    for library, (unit, _) in LIBRARIES.items():
+    for library, (units, _) in LIBRARIES.items():
         if not force and not _library_is_stale(library):
             continue
         tmp = library.with_suffix('.so.tmp')
-        cmd = [nvcc_path(), *NVCC_FLAGS, '-I', str(INCLUDE_DIR), '-o', str(tmp), str(unit)]
+        cmd = [nvcc_path(), *NVCC_FLAGS, '-I', str(INCLUDE_DIR), '--threads', str(len(units)),
+               '-o', str(tmp), *map(str, units)]
         if verbose:
             cmd.insert(1, '-Xptxas=-v')
             print(' '.join(cmd), file=sys.stderr)

@@ -2,16 +2,17 @@
 #include "mvquant.h"
 
 #include <cmath>
+#include <cstdlib>
 #include <cstdarg>
 #include <cstdio>
 #include <mutex>
 
+#include "mvq_host.cuh"
 #include "quant_rows.cuh"
-#include "w4_linear.cuh"
 
-namespace {
+namespace mvq {
 
-thread_local char g_error[512];
+static thread_local char g_error[512];
 
 int fail(int code, const char* fmt, ...) {
     va_list args;
@@ -25,7 +26,14 @@ int cuda_fail(cudaError_t err, const char* what) {
     return fail(MVQ_ERR_CUDA, "%s: %s", what, cudaGetErrorString(err));
 }
 
-constexpr int kMaxDevices = 64;
+}  // namespace mvq
+
+namespace {
+
+using mvq::cuda_fail;
+using mvq::fail;
+using mvq::launch;
+using mvq::kMaxDevices;
 
 // Streaming multiprocessors of the current device (asked once per device).
 int device_sms(int* device, int* sms) {
@@ -49,28 +57,6 @@ bool float_dtype(int64_t d) { return d == MVQ_DTYPE_F32 || d == MVQ_DTYPE_F16 ||
 int64_t dtype_size(int64_t d) { return d == MVQ_DTYPE_F32 ? 4 : d == MVQ_DTYPE_F16 || d == MVQ_DTYPE_BF16 ? 2 : 1; }
 uintptr_t address(const void* p) { return reinterpret_cast<uintptr_t>(p); }
 
-// Programmatic stream serialization (the kernels wait before they read), and a
-// cluster along x where one is asked for.
-template <typename... Params, typename... Args>
-cudaError_t launch(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, int cluster, void* stream,
-                   Args&&... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = static_cast<cudaStream_t>(stream);
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = cluster;
-    attr[1].val.clusterDim.y = 1;
-    attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = cluster > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
-}
-
 // ------------------------------------------------------------------- weights
 
 constexpr int64_t kMaxSize = int64_t(1) << 30;
@@ -85,65 +71,6 @@ int check_weight(const void* records, int64_t n, int64_t k, int64_t group, int64
     if (scale_dtype != MVQ_DTYPE_F16 && scale_dtype != MVQ_DTYPE_BF16)
         return fail(MVQ_ERR_INVALID_ARGUMENT, "scale_dtype must be MVQ_DTYPE_F16 or MVQ_DTYPE_BF16");
     return MVQ_OK;
-}
-
-int record_bytes(int64_t group, int64_t has_zeros) {
-    return mvq::kCodeBytes + static_cast<int>(mvq::kChunk / group) * (has_zeros ? 192 : 128);
-}
-
-template <int XT, int NB, int GROUP>
-int launch_linear(const mvq::LinearParams& p, int device, int tiles, int blocks, void* stream) {
-    auto kernel = mvq::w4_linear_kernel<XT, NB, GROUP>;
-    constexpr int kMost = mvq::kWarps * mvq::kStages * (mvq::kCodeBytes + mvq::kChunk / GROUP * 192);
-    static std::mutex mutex;
-    static bool ready[kMaxDevices];
-    {
-        std::lock_guard<std::mutex> lock(mutex);
-        if (!ready[device]) {
-            cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
-            if (err == cudaSuccess)
-                err = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
-                                           static_cast<int>(cudaSharedmemCarveoutMaxShared));
-            if (err != cudaSuccess) return cuda_fail(err, "cudaFuncSetAttribute");
-            ready[device] = true;
-        }
-    }
-    const size_t smem = static_cast<size_t>(mvq::kWarps) * mvq::kStages * p.record_bytes;
-    const dim3 grid(static_cast<unsigned>(tiles) * p.cluster, blocks);
-    const cudaError_t err = launch(kernel, grid, mvq::kThreads, smem, p.cluster, stream, p);
-    return err == cudaSuccess ? MVQ_OK : cuda_fail(err, "4-bit linear kernel launch");
-}
-
-template <int XT, int NB>
-int launch_linear_group(const mvq::LinearParams& p, int64_t group, int device, int tiles, int blocks, void* stream) {
-    switch (group) {
-        case 32: return launch_linear<XT, NB, 32>(p, device, tiles, blocks, stream);
-        case 64: return launch_linear<XT, NB, 64>(p, device, tiles, blocks, stream);
-        default: return launch_linear<XT, NB, 128>(p, device, tiles, blocks, stream);
-    }
-}
-
-template <int XT>
-int launch_linear_tokens(const mvq::LinearParams& p, int64_t group, int device, int sms, int tiles, void* stream) {
-    // Tokens per pass over the records: 8, 16 or 32 (fp32 x is three numbers per element: 8).
-    const int most = XT == mvq::kF32 ? 1 : 4;
-    int nb = p.m <= 8 ? 1 : p.m <= 16 ? 2 : 4;
-    if (nb > most) nb = most;
-    const int64_t blocks = (static_cast<int64_t>(p.m) + 8 * nb - 1) / (8 * nb);
-    if (blocks > 65535) return fail(MVQ_ERR_UNSUPPORTED, "too many rows of x for one call");
-    mvq::LinearParams q = p;
-    q.cluster = 1;
-    while (q.cluster < 8 && static_cast<int64_t>(tiles) * blocks * q.cluster < 3 * static_cast<int64_t>(sms) &&
-           p.chunks > mvq::kWarps * q.cluster)
-        q.cluster *= 2;
-    if (static_cast<int64_t>(tiles) * q.cluster >= (int64_t(1) << 31))
-        return fail(MVQ_ERR_UNSUPPORTED, "too many weight rows for one call");
-    const int b = static_cast<int>(blocks);
-    if constexpr (XT != mvq::kF32) {
-        if (nb == 4) return launch_linear_group<XT, 4>(q, group, device, tiles, b, stream);
-        if (nb == 2) return launch_linear_group<XT, 2>(q, group, device, tiles, b, stream);
-    }
-    return launch_linear_group<XT, 1>(q, group, device, tiles, b, stream);
 }
 
 // ---------------------------------------------------------------------- rows
@@ -218,7 +145,7 @@ extern "C" {
 
 int mvq_abi_version(void) { return MVQ_ABI_VERSION; }
 
-const char* mvq_last_error(void) { return g_error; }
+const char* mvq_last_error(void) { return mvq::g_error; }
 
 int mvq_w4_linear(const MvqLinearArgs* a, void* stream) try {
     if (!a) return fail(MVQ_ERR_INVALID_ARGUMENT, "args must not be NULL");
@@ -247,8 +174,8 @@ int mvq_w4_linear(const MvqLinearArgs* a, void* stream) try {
     p.k = static_cast<int>(a->k);
     p.m = static_cast<int>(a->m);
     p.chunks = static_cast<int>((a->k + mvq::kChunk - 1) / mvq::kChunk);
-    p.record_bytes = record_bytes(a->group, a->has_zeros);
-    p.has_zeros = a->has_zeros != 0;
+    p.tiles = static_cast<int>((a->n + mvq::kTileRows - 1) / mvq::kTileRows);
+    p.x_dtype = static_cast<int>(a->x_dtype);
     p.scale_bf16 = a->scale_dtype == MVQ_DTYPE_BF16;
     p.x_runs = a->k % 8 == 0 && address(a->x) % run == 0 && (a->m == 1 || a->x_stride_row * size % run == 0);
     p.bias = a->bias;
@@ -257,14 +184,18 @@ int mvq_w4_linear(const MvqLinearArgs* a, void* stream) try {
     p.out = a->out;
     p.out_stride = a->out_stride_row;
     p.out_dtype = static_cast<int>(a->out_dtype);
-    const int tiles = static_cast<int>((a->n + mvq::kTileRows - 1) / mvq::kTileRows);
-    switch (a->x_dtype) {
-        case MVQ_DTYPE_F32: return launch_linear_tokens<mvq::kF32>(p, a->group, device, sms, tiles, stream);
-        case MVQ_DTYPE_F16: return launch_linear_tokens<mvq::kF16>(p, a->group, device, sms, tiles, stream);
-        case MVQ_DTYPE_BF16: return launch_linear_tokens<mvq::kBF16>(p, a->group, device, sms, tiles, stream);
-        case MVQ_DTYPE_I8: return launch_linear_tokens<mvq::kI8>(p, a->group, device, sms, tiles, stream);
-        default: return launch_linear_tokens<mvq::kE4M3>(p, a->group, device, sms, tiles, stream);
-    }
+    p.x_units = a->x_dtype == MVQ_DTYPE_I8 ? p.x_runs && a->k % 16 == 0 && address(a->x) % 16 == 0 &&
+                                                 (a->m == 1 || a->x_stride_row % 16 == 0)
+                                           : p.x_runs && size == 2;
+    const int kind = a->x_dtype == MVQ_DTYPE_E4M3 ? mvq::kF16 : static_cast<int>(a->x_dtype);
+    const int group = static_cast<int>(a->group);
+    int few = 8;
+#ifdef MVQ_TUNE
+    if (getenv("FEW")) few = atoi(getenv("FEW"));
+#endif
+    if (kind == mvq::kF32 || a->m <= few)
+        return mvq::launch_narrow(p, kind, group, a->has_zeros != 0, device, sms, stream);
+    return mvq::launch_wide(p, kind, group, a->has_zeros != 0, device, sms, stream);
 } catch (...) {
     return fail(MVQ_ERR_CUDA, "unexpected C++ exception");
 }
@@ -284,7 +215,7 @@ int mvq_w4_dequantize(const MvqDequantizeArgs* a, void* stream) try {
     const int64_t size = dtype_size(a->out_dtype);
     const int runs = address(a->out) % 16 == 0 && (a->n == 1 || a->out_stride_row * size % 16 == 0);
     const dim3 grid(static_cast<unsigned>((total + 7) / 8));
-    const int bytes = record_bytes(a->group, a->has_zeros), bf16 = a->scale_dtype == MVQ_DTYPE_BF16;
+    const int bytes = mvq::record_size(static_cast<int>(a->group), a->has_zeros != 0), bf16 = a->scale_dtype == MVQ_DTYPE_BF16;
     const uint8_t* records = static_cast<const uint8_t*>(a->records);
     const int group = static_cast<int>(a->group), zeros = a->has_zeros != 0;
     const int n = static_cast<int>(a->n), k = static_cast<int>(a->k);

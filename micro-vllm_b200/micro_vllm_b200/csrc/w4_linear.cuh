@@ -31,11 +31,12 @@ constexpr int kChunk = 128;
 constexpr int kCodeBytes = kTileRows * kChunk / 2;
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kStages = 4;
 // Row stride of the partial sums [token][64 weight rows] in shared memory, in
 // floats: 68 keeps the eight rows and four token pairs that a warp stores at
 // once in different banks.
 constexpr int kPartStride = 68;
+
+__host__ __device__ constexpr int record_size(int group, bool zeros) { return kCodeBytes + kChunk / group * (zeros ? 192 : 128); }
 
 struct LinearParams {
     const void* x;
@@ -44,11 +45,16 @@ struct LinearParams {
     const uint8_t* records;
     int n, k, m;
     int chunks;        // ceil(k / 128)
-    int record_bytes;
-    int has_zeros;
+    int tiles;         // ceil(n / 64)
     int scale_bf16;
+    int x_dtype;
     int x_runs;        // x may be read 8 elements at a time: aligned rows, k a multiple of 8
-    int cluster;       // CTAs that share a tile's columns
+    int x_units;       // x may be copied in units of 16 bytes as it is
+    int cluster;       // CTAs that share a tile's columns, each with a run of chunks
+    int ksplit;        // warps of a CTA that share a tile's columns: its kWarps / ksplit tiles
+    int stages;        // records in flight per warp
+    int x_chunks;      // chunks of x staged at a time (a multiple of ksplit)
+    int ring_bytes;    // shared memory of a warp: its records, later its partial sums
     const void* bias;
     const void* residual;
     int64_t residual_stride;
@@ -96,23 +102,22 @@ __device__ __forceinline__ float2 scale_pair(uint32_t bits, int bf16) {
     return __half22float2(*reinterpret_cast<const __half2*>(&bits));
 }
 
-// Operand arithmetic of each activation type. A holds how a word of codes
-// (rows g and g + 8 of a 16-row block, columns 4e..4e+3 of the lane's run of
-// eight) becomes operand registers; kPlanes bf16 numbers make up one x.
-template <int XT>
+// Operand arithmetic of each kind of product: kPlanes operand numbers make up
+// one x, kRunBytes hold eight of them for the B operand, and weights() makes
+// the A registers of a word of codes (rows g and g + 8 of 16 rows, four columns).
+template <int KIND>
 struct Act;
 
-struct ActHalfBase {
-    static constexpr int kRegs = 4;  // 32-bit registers of x per plane, 8-column run and token
+struct ActHalf {
+    static constexpr int kPlanes = 1;
+    static constexpr int kRunBytes = 16;
 };
 
 template <>
-struct Act<kBF16> : ActHalfBase {
-    using T = __nv_bfloat16;
-    static constexpr int kPlanes = 1;
+struct Act<kBF16> : ActHalf {
     // (code - zero) / 2^11 from 128 + code (bf16 numbers from 128 to 255 have a
     // step of one): (128 + code) / 2^11 - (128 + zero) / 2^11, exact. The power
-    // of two goes back into the scale; with it a group's sum of 128 products of
+    // of two (kScale) comes back after the sum; with it a group's sum of 128 products of
     // at most 15 stays below the largest |x|, so no x that is finite overflows.
     static constexpr float kScale = 2048.0f;
     __device__ __forceinline__ static uint32_t zero_low(int z) { return (0xbd80u + z) * 0x10001u; }
@@ -133,19 +138,24 @@ struct Act<kBF16> : ActHalfBase {
     __device__ __forceinline__ static void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
         mv::MmaOp<__nv_bfloat16>::run(c, a, b0, b1);
     }
+    // c = a b, without a register to be cleared first.
+    __device__ __forceinline__ static void mma_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, "
+            "{%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+    }
 };
 
 // fp32 x as the exact sum of three bf16 numbers (8 + 8 + 8 bits of its 24).
 template <>
 struct Act<kF32> : Act<kBF16> {
-    using T = float;
     static constexpr int kPlanes = 3;
 };
 
 template <>
-struct Act<kF16> : ActHalfBase {
-    using T = __half;
-    static constexpr int kPlanes = 1;
+struct Act<kF16> : ActHalf {
     static constexpr float kScale = 1.0f;
     // Low nibbles become 1024 + code (step one), high nibbles 1024 + 16 code,
     // then code - zero as (1024 + 16 code) / 16 - (64 + zero): all exact.
@@ -171,20 +181,28 @@ struct Act<kF16> : ActHalfBase {
     __device__ __forceinline__ static void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
         mv::MmaOp<__half>::run(c, a, b0, b1);
     }
-};
-
-// e4m3 numbers are exact in fp16.
-template <>
-struct Act<kE4M3> : Act<kF16> {
-    using T = __nv_fp8_storage_t;
+    __device__ __forceinline__ static void mma_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
+            "{%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+    }
 };
 
 template <>
 struct Act<kI8> {
-    using T = int8_t;
     static constexpr int kPlanes = 1;
-    static constexpr int kRegs = 2;
+    static constexpr int kRunBytes = 8;
+    // A nibble (code - 8 in two's complement) in a byte's high half is 16 (code - 8).
+    static constexpr float kScale = 1.0f / 16.0f;
 };
+
+// The four columns of a word as int8 (code - zero), rows g and g + 8. Bytes 128 +
+// code minus bytes zero borrow nothing from one another; then 128 is taken off.
+__device__ __forceinline__ uint32_t bytes_minus(uint32_t w, uint32_t zero4) {
+    return (and_xor(w, 0x0f0f0f0fu, 0x88888888u) - zero4) ^ 0x80808080u;
+}
 
 __device__ __forceinline__ void mma_s8(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -194,32 +212,22 @@ __device__ __forceinline__ void mma_s8(int (&c)[4], const uint32_t (&a)[4], uint
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Eight consecutive elements of a row of x as operand registers: columns k..k+7
-// (zeros at and beyond `limit`), r[plane][...]. `runs`: one vector load.
-template <int XT>
-__device__ __forceinline__ void load_run(const typename Act<XT>::T* row, int k, int limit, bool runs,
-                                         uint32_t (&r)[Act<XT>::kPlanes][Act<XT>::kRegs]) {
-    if constexpr (XT == kBF16 || XT == kF16) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (runs) {
-            if (k < limit) v = __ldg(reinterpret_cast<const uint4*>(row + k));
-        } else {
-            const uint16_t* e = reinterpret_cast<const uint16_t*>(row);
-            uint32_t h[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) h[i] = k + i < limit ? __ldg(e + k + i) : 0u;
-            v = make_uint4(h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16));
-        }
-        r[0][0] = v.x, r[0][1] = v.y, r[0][2] = v.z, r[0][3] = v.w;
-    } else if constexpr (XT == kF32) {
+// Eight consecutive elements of a row of x, columns k..k+7 (zeros at and beyond
+// `limit`), as operand numbers of kind KIND: r[plane][...] holds them in order,
+// two to a register (int8: four). e4m3 numbers are exact in fp16.
+template <int KIND>
+__device__ __forceinline__ void load_run(const LinearParams& p, const void* row, int k, int limit,
+                                         uint32_t (&r)[Act<KIND>::kPlanes][Act<KIND>::kRunBytes / 4]) {
+    if constexpr (KIND == kF32) {
+        const float* e = static_cast<const float*>(row);
         float f[8];
-        if (runs && k < limit) {
-            const float4 lo = __ldg(reinterpret_cast<const float4*>(row + k));
-            const float4 hi = __ldg(reinterpret_cast<const float4*>(row + k) + 1);
+        if (p.x_runs && k < limit) {
+            const float4 lo = *reinterpret_cast<const float4*>(e + k);
+            const float4 hi = *reinterpret_cast<const float4*>(e + k + 4);
             f[0] = lo.x, f[1] = lo.y, f[2] = lo.z, f[3] = lo.w, f[4] = hi.x, f[5] = hi.y, f[6] = hi.z, f[7] = hi.w;
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = k + i < limit ? __ldg(row + k + i) : 0.0f;
+            for (int i = 0; i < 8; ++i) f[i] = k + i < limit ? e[k + i] : 0.0f;
         }
         // Truncation to bf16 three times: x = b0 + b1 + b2 exactly. What is not
         // finite goes into b0 alone (a NaN may not lose its last bits to an infinity).
@@ -233,24 +241,36 @@ __device__ __forceinline__ void load_run(const typename Act<XT>::T* row, int k, 
             b[2][i] = __float_as_uint(rest - __uint_as_float(b[1][i])) & 0xffff0000u;
         }
 #pragma unroll
-        for (int p = 0; p < 3; ++p)
+        for (int pl = 0; pl < 3; ++pl)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) r[p][i] = (b[p][2 * i] >> 16) | b[p][2 * i + 1];
-    } else {
-        uint2 v = make_uint2(0, 0);
-        const uint8_t* e = reinterpret_cast<const uint8_t*>(row);
-        if (runs) {
-            if (k < limit) v = __ldg(reinterpret_cast<const uint2*>(e + k));
+            for (int i = 0; i < 4; ++i) r[pl][i] = (b[pl][2 * i] >> 16) | b[pl][2 * i + 1];
+    } else if (KIND != kI8 && p.x_dtype != kE4M3) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        const uint16_t* e = static_cast<const uint16_t*>(row);
+        if (p.x_runs) {
+            if (k < limit) v = *reinterpret_cast<const uint4*>(e + k);
         } else {
             uint32_t h[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) h[i] = k + i < limit ? __ldg(e + k + i) : 0u;
+            for (int i = 0; i < 8; ++i) h[i] = k + i < limit ? e[k + i] : 0u;
+            v = make_uint4(h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16));
+        }
+        r[0][0] = v.x, r[0][1] = v.y;
+        if constexpr (Act<KIND>::kRunBytes == 16) r[0][2] = v.z, r[0][3] = v.w;
+    } else {
+        uint2 v = make_uint2(0, 0);
+        const uint8_t* e = static_cast<const uint8_t*>(row);
+        if (p.x_runs) {
+            if (k < limit) v = *reinterpret_cast<const uint2*>(e + k);
+        } else {
+            uint32_t h[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) h[i] = k + i < limit ? e[k + i] : 0u;
             v = make_uint2(h[0] | (h[1] << 8) | (h[2] << 16) | (h[3] << 24),
                            h[4] | (h[5] << 8) | (h[6] << 16) | (h[7] << 24));
         }
-        if constexpr (XT == kI8) {  // the codes' byte order: 0, 2, 1, 3
-            r[0][0] = __byte_perm(v.x, 0, 0x3120);
-            r[0][1] = __byte_perm(v.y, 0, 0x3120);
+        if constexpr (KIND == kI8) {
+            r[0][0] = v.x, r[0][1] = v.y;
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -292,60 +312,88 @@ __device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
     return v;
 }
 
-// One cluster of `cluster` CTAs per (tile of 64 weight rows, block of 8 NB
-// tokens). The chunks of 128 columns are dealt to its 4 * cluster warps in
-// turn; each warp streams its records through a ring of its own (cp.async, no
-// barrier: the warp reads what its own lanes copied), sums all 64 rows for all
-// its tokens, and the warps' partial sums meet in (distributed) shared memory,
-// added in a fixed order.
-template <int XT, int NB, int GROUP>
-__global__ void __launch_bounds__(kThreads) w4_linear_kernel(const LinearParams p) {
-    using A = Act<XT>;
-    using T = typename A::T;
-    constexpr int kGroupRuns = GROUP / 32;        // 32-column runs per group
-    constexpr int kGroups = kChunk / GROUP;       // groups per chunk
+// A CTA's four warps take 4 / ksplit tiles of 64 weight rows and, with the other
+// CTAs of their cluster, a block of 8 NB tokens. The columns' chunks go to the
+// cluster's CTAs as runs, within a CTA to the tile's ksplit warps in turn. x's
+// part of the run is staged in shared memory once, as operand numbers; each warp
+// streams its records through a ring of its own (cp.async and no barrier: a warp
+// reads what its own lanes copied) and sums all 64 rows for all tokens; the
+// partial sums meet in (distributed) shared memory and are added in a fixed order.
+template <int KIND, int NB, int GROUP, bool ZEROS>
+__global__ void __launch_bounds__(kThreads, NB == 4 ? 2 : 4) w4_linear_kernel(const LinearParams p) {
+    using A = Act<KIND>;
+    constexpr int kGroupRuns = GROUP / 32;    // 32-column runs per group
+    constexpr int kGroups = kChunk / GROUP;   // groups per chunk
+    constexpr int kRecord = record_size(GROUP, ZEROS);
+    constexpr int kPlanes = A::kPlanes, kRunBytes = A::kRunBytes;
     extern __shared__ __align__(128) uint8_t smem[];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
-    const uint32_t rank = p.cluster > 1 ? cluster_rank() : 0;
-    const int64_t tile = blockIdx.x / p.cluster;
+    const int rank = p.cluster > 1 ? static_cast<int>(cluster_rank()) : 0;
+    const int64_t tile0 = static_cast<int64_t>(blockIdx.x) / p.cluster * (kWarps / p.ksplit);
+    const int64_t tile = tile0 + warp / p.ksplit;
     const int token0 = blockIdx.y * (8 * NB);
-    const int step = kWarps * p.cluster;
-    const int first = static_cast<int>(rank) * kWarps + warp;
-    const int mine = p.chunks > first ? (p.chunks - first + step - 1) / step : 0;
-    const uint8_t* base = p.records + tile * p.chunks * static_cast<int64_t>(p.record_bytes);
-    const uint32_t ring = mv::smem_addr(smem) + warp * kStages * p.record_bytes;
+    const int tokens = min(8 * NB, p.m - token0);
+    // This CTA's run of chunks, and this warp's among them: begin + kpart, + ksplit, ...
+    const int begin = static_cast<int>(static_cast<int64_t>(p.chunks) * rank / p.cluster);
+    const int end = static_cast<int>(static_cast<int64_t>(p.chunks) * (rank + 1) / p.cluster);
+    const int kpart = warp % p.ksplit;
+    const int mine = tile < p.tiles && end - begin > kpart ? (end - begin - kpart + p.ksplit - 1) / p.ksplit : 0;
+    const uint8_t* base = p.records + (tile * p.chunks + begin + kpart) * static_cast<int64_t>(kRecord);
+    const int64_t base_step = static_cast<int64_t>(p.ksplit) * kRecord;
+    const uint32_t ring = mv::smem_addr(smem) + warp * p.ring_bytes;
+    uint8_t* const xs = smem + kWarps * p.ring_bytes;
 
     // The weights' first records come into L2 while the grid before drains. Its
     // writes are not visible yet, so nothing is read.
-    for (int i = 0; i < kStages && i < mine; ++i) {
-        const uint8_t* rec = base + static_cast<int64_t>(first + i * step) * p.record_bytes;
-        for (int b = lane * 128; b < p.record_bytes; b += 32 * 128)
-            asm volatile("prefetch.global.L2 [%0];" ::"l"(rec + b));
-    }
+    for (int i = 0; i < p.stages && i < mine; ++i)
+        for (int b = lane * 128; b < kRecord; b += 32 * 128)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(base + i * base_step + b));
     mv::wait_for_prior_grid();
     mv::allow_next_grid();
 
-    auto issue = [&](int i) {
+    int fill = 0;  // stage that the next record goes to
+    const auto issue = [&](int i) {
         if (i < mine) {
-            const uint8_t* rec = base + static_cast<int64_t>(first + i * step) * p.record_bytes;
-            const uint32_t dst = ring + (i % kStages) * p.record_bytes;
-            for (int b = lane * 16; b < p.record_bytes; b += 32 * 16) cp_async_16(dst + b, rec + b);
+            const uint8_t* rec = base + i * base_step + lane * 16;
+            const uint32_t dst = ring + fill * kRecord + lane * 16;
+#pragma unroll
+            for (int b = 0; b < kRecord; b += 512)
+                if (b + 512 <= kRecord || b + lane * 16 < kRecord) cp_async_16(dst + b, rec + b);
         }
         cp_async_commit();
+        fill = fill + 1 == p.stages ? 0 : fill + 1;
     };
-#pragma unroll
-    for (int i = 0; i < kStages; ++i) issue(i);
+    for (int i = 0; i < p.stages; ++i) issue(i);
 
-    const T* rows[NB];
-    bool live[NB];
+    // x: [chunk][h][plane][t][token] two quads, the columns 16 e + 4 t of h, for x_chunks chunks from `from`.
+    const int plane_bytes = 4 * tokens * kRunBytes;
+    const int x_size = p.x_dtype == kF32 ? 4 : p.x_dtype >= kI8 ? 1 : 2;
+    const auto stage_x = [&](int from) {
+        const int runs = min(p.x_chunks, end - begin - from) * 16;  // runs of eight of a token: chunk, h, t
+        for (int token = 0; token < tokens; ++token) {
+            const uint8_t* row = static_cast<const uint8_t*>(p.x) + (token0 + token) * p.x_stride * x_size;
+            for (int run = threadIdx.x; run < runs; run += kThreads) {
+                uint32_t r[kPlanes][kRunBytes / 4];
+                load_run<KIND>(p, row, (begin + from) * kChunk + run * 8, p.k, r);
+                // The run's two quads go to lanes t = 2 (run & 1) and the next, as their columns 16 e + 4 t..
+                uint8_t* dst = xs + (run >> 2) * (kPlanes * plane_bytes) +
+                               ((run & 1) * 2 * tokens + token) * kRunBytes + (run >> 1 & 1) * (kRunBytes / 2);
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        const int token = token0 + 8 * b + g;
-        live[b] = token < p.m;
-        rows[b] = static_cast<const T*>(p.x) + (live[b] ? token : 0) * p.x_stride;
-    }
+                for (int pl = 0; pl < kPlanes; ++pl) {
+                    uint8_t* d = dst + pl * plane_bytes;
+                    if constexpr (KIND == kI8) {  // the codes' byte order: 0, 2, 1, 3
+                        *reinterpret_cast<uint32_t*>(d) = __byte_perm(r[0][0], 0, 0x3120);
+                        *reinterpret_cast<uint32_t*>(d + tokens * kRunBytes) = __byte_perm(r[0][1], 0, 0x3120);
+                    } else {
+                        *reinterpret_cast<uint2*>(d) = make_uint2(r[pl][0], r[pl][1]);
+                        *reinterpret_cast<uint2*>(d + tokens * kRunBytes) = make_uint2(r[pl][2], r[pl][3]);
+                    }
+                }
+            }
+        }
+    };
 
     float acc[4][NB][4];
 #pragma unroll
@@ -355,64 +403,84 @@ __global__ void __launch_bounds__(kThreads) w4_linear_kernel(const LinearParams 
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[r][b][e] = 0.0f;
 
-    for (int i = 0; i < mine; ++i) {
-        const int k0 = (first + i * step) * kChunk;
-        uint32_t x[4][NB][A::kPlanes][A::kRegs];
+    // A lane of a token beyond the last reads the last: its column of the product is never stored.
+    const uint32_t x_lane = mv::smem_addr(xs) + t * tokens * kRunBytes;
+    uint32_t x_token[NB];
 #pragma unroll
-        for (int h = 0; h < 4; ++h)
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-                load_run<XT>(rows[b], k0 + 32 * h + 8 * t, live[b] ? p.k : 0, p.x_runs, x[h][b]);
-        cp_async_wait<kStages - 1>();
+    for (int b = 0; b < NB; ++b) x_token[b] = min(8 * b + g, tokens - 1) * kRunBytes;
+    int drain = 0;  // stage of the record that is read next
+    for (int from = 0; from < end - begin; from += p.x_chunks) {
+    if (from) __syncthreads();  // every warp is done with the chunks of x before
+    stage_x(from);
+    __syncthreads();
+    const int last = min(mine, (from + p.x_chunks) / p.ksplit);
+    for (int i = from / p.ksplit; i < last; ++i) {
+        if (p.stages == 2) cp_async_wait<1>();
+        else if (p.stages == 3) cp_async_wait<2>();
+        else cp_async_wait<3>();
         __syncwarp();
-        const uint32_t rec = ring + (i % kStages) * p.record_bytes;
+        const uint32_t rec = ring + drain * kRecord;
+        drain = drain + 1 == p.stages ? 0 : drain + 1;
         const uint32_t scales = rec + kCodeBytes + g * 16;
         const uint32_t zeros = rec + kCodeBytes + kGroups * 128 + g * 8;
+        const uint32_t x_chunk = x_lane + (i * p.ksplit + kpart - from) * (4 * kPlanes * plane_bytes);
 #pragma unroll
         for (int rp = 0; rp < 2; ++rp) {  // 32 rows at a time
-            if constexpr (XT == kI8) {
-                int c[2][NB][4], sum[NB][4];
+            if constexpr (KIND == kI8) {
+                // Sums start at 1.5 2^23 as a float's bits: their float value is then one subtraction away,
+                // as they stay below 2^22 (16 * 8 * 128 * 128, or 15 * 128 * 128 with zero points).
+                constexpr int kBias = 0x4b400000;
+                int c[2][NB][4];
+                uint32_t zl[2], zh[2];
 #pragma unroll
                 for (int h = 0; h < 4; ++h) {
                     if (h % kGroupRuns == 0) {
 #pragma unroll
                         for (int b = 0; b < NB; ++b)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) c[0][b][e] = c[1][b][e] = sum[b][e] = 0;
+                            for (int e = 0; e < 4; ++e) c[0][b][e] = c[1][b][e] = kBias;
+                        if constexpr (ZEROS) {
+                            // zero - 8 as a byte, plus 8, in all four bytes of an operand.
+                            const uint32_t z = lds32(zeros + (h / kGroupRuns) * 64 + rp * 4) ^ 0x88888888u;
+                            const uint32_t u = (z & 0x0f0f0f0fu);
+#pragma unroll
+                            for (int q = 0; q < 2; ++q) {
+                                zl[q] = __byte_perm(u, 0, q ? 0x2222 : 0x0000);
+                                zh[q] = __byte_perm(u, 0, q ? 0x3333 : 0x1111);
+                            }
+                        }
                     }
                     const uint4 w = lds128(rec + ((h * 2 + rp) * 32 + lane) * 16);
-                    // A nibble (code - 8 in two's complement) in a byte's high half is 16 (code - 8).
-                    const uint32_t a0[4] = {(w.x << 4) & 0xf0f0f0f0u, w.x & 0xf0f0f0f0u, (w.y << 4) & 0xf0f0f0f0u,
-                                            w.y & 0xf0f0f0f0u};
-                    const uint32_t a1[4] = {(w.z << 4) & 0xf0f0f0f0u, w.z & 0xf0f0f0f0u, (w.w << 4) & 0xf0f0f0f0u,
-                                            w.w & 0xf0f0f0f0u};
-                    const uint32_t ones[4] = {0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u};
+                    uint32_t a0[4], a1[4];
+                    if constexpr (ZEROS) {
+                        a0[0] = bytes_minus(w.x, zl[0]), a0[1] = bytes_minus(w.x >> 4, zh[0]);
+                        a0[2] = bytes_minus(w.y, zl[0]), a0[3] = bytes_minus(w.y >> 4, zh[0]);
+                        a1[0] = bytes_minus(w.z, zl[1]), a1[1] = bytes_minus(w.z >> 4, zh[1]);
+                        a1[2] = bytes_minus(w.w, zl[1]), a1[3] = bytes_minus(w.w >> 4, zh[1]);
+                    } else {
+                        a0[0] = (w.x << 4) & 0xf0f0f0f0u, a0[1] = w.x & 0xf0f0f0f0u;
+                        a0[2] = (w.y << 4) & 0xf0f0f0f0u, a0[3] = w.y & 0xf0f0f0f0u;
+                        a1[0] = (w.z << 4) & 0xf0f0f0f0u, a1[1] = w.z & 0xf0f0f0f0u;
+                        a1[2] = (w.w << 4) & 0xf0f0f0f0u, a1[3] = w.w & 0xf0f0f0f0u;
+                    }
 #pragma unroll
                     for (int b = 0; b < NB; ++b) {
-                        mma_s8(c[0][b], a0, x[h][b][0][0], x[h][b][0][1]);
-                        mma_s8(c[1][b], a1, x[h][b][0][0], x[h][b][0][1]);
-                        if (p.has_zeros) mma_s8(sum[b], ones, x[h][b][0][0], x[h][b][0][1]);
+                        const uint2 xv = lds64(x_chunk + h * plane_bytes + x_token[b]);
+                        mma_s8(c[0][b], a0, xv.x, xv.y);
+                        mma_s8(c[1][b], a1, xv.x, xv.y);
                     }
                     if (h % kGroupRuns == kGroupRuns - 1) {
-                        const int group = h / kGroupRuns;
-                        const uint2 s = lds64(scales + group * 128 + rp * 8);
-                        uint32_t z = 0;
-                        if (p.has_zeros) z = lds32(zeros + group * 64 + rp * 4);
+                        const uint2 s = lds64(scales + (h / kGroupRuns) * 128 + rp * 8);
 #pragma unroll
                         for (int q = 0; q < 2; ++q) {
                             const float2 sc = scale_pair(q ? s.y : s.x, p.scale_bf16);
-                            const int zl = 16 * static_cast<int8_t>(z >> (16 * q));
-                            const int zh = 16 * static_cast<int8_t>(z >> (16 * q + 8));
-                            const float lo = sc.x * 0.0625f, hi = sc.y * 0.0625f;
 #pragma unroll
-                            for (int b = 0; b < NB; ++b) {
-                                // Below 2^24 (16 * 15 * 128 * 128): exact as floats.
-                                float(&a)[4] = acc[2 * rp + q][b];
-                                a[0] = fmaf(lo, static_cast<float>(c[q][b][0] - zl * sum[b][0]), a[0]);
-                                a[1] = fmaf(lo, static_cast<float>(c[q][b][1] - zl * sum[b][1]), a[1]);
-                                a[2] = fmaf(hi, static_cast<float>(c[q][b][2] - zh * sum[b][2]), a[2]);
-                                a[3] = fmaf(hi, static_cast<float>(c[q][b][3] - zh * sum[b][3]), a[3]);
-                            }
+                            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    acc[2 * rp + q][b][e] =
+                                        fmaf(e < 2 ? sc.x : sc.y, __int_as_float(c[q][b][e]) - 12582912.0f,
+                                             acc[2 * rp + q][b][e]);
                         }
                     }
                 }
@@ -423,17 +491,20 @@ __global__ void __launch_bounds__(kThreads) w4_linear_kernel(const LinearParams 
                 for (int h = 0; h < 4; ++h) {
                     if (h % kGroupRuns == 0) {
                         uint32_t z = 0;
-                        if (p.has_zeros) z = lds32(zeros + (h / kGroupRuns) * 64 + rp * 4);
+                        if (ZEROS) z = lds32(zeros + (h / kGroupRuns) * 64 + rp * 4);
 #pragma unroll
                         for (int q = 0; q < 2; ++q) {
                             zl[q] = A::zero_low(8 + static_cast<int8_t>(z >> (16 * q)));
                             zh[q] = A::zero_high(8 + static_cast<int8_t>(z >> (16 * q + 8)));
-#pragma unroll
-                            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) c[q][b][e] = 0.0f;
                         }
                     }
+                    uint4 xv[NB][kPlanes];
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+#pragma unroll
+                        for (int pl = 0; pl < kPlanes; ++pl) {
+                            xv[b][pl] = lds128(x_chunk + (h * kPlanes + pl) * plane_bytes + x_token[b]);
+                        }
                     const uint4 w = lds128(rec + ((h * 2 + rp) * 32 + lane) * 16);
                     const uint32_t words[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -443,62 +514,85 @@ __global__ void __launch_bounds__(kThreads) w4_linear_kernel(const LinearParams 
 #pragma unroll
                         for (int b = 0; b < NB; ++b)
 #pragma unroll
-                            for (int pl = 0; pl < A::kPlanes; ++pl)
-                                A::mma(c[j >> 1][b], a, x[h][b][pl][2 * (j & 1)], x[h][b][pl][2 * (j & 1) + 1]);
+                            for (int pl = 0; pl < kPlanes; ++pl) {
+                                const uint32_t b0 = j & 1 ? xv[b][pl].z : xv[b][pl].x;
+                                const uint32_t b1 = j & 1 ? xv[b][pl].w : xv[b][pl].y;
+                                if (h % kGroupRuns == 0 && (j & 1) == 0 && pl == 0) A::mma_first(c[j >> 1][b], a, b0, b1);
+                                else A::mma(c[j >> 1][b], a, b0, b1);
+                            }
                     }
                     if (h % kGroupRuns == kGroupRuns - 1) {
                         const uint2 s = lds64(scales + (h / kGroupRuns) * 128 + rp * 8);
 #pragma unroll
                         for (int q = 0; q < 2; ++q) {
-                            float2 sc = scale_pair(q ? s.y : s.x, p.scale_bf16);
-                            sc.x *= A::kScale, sc.y *= A::kScale;
+                            const float2 sc = scale_pair(q ? s.y : s.x, p.scale_bf16);
 #pragma unroll
-                            for (int b = 0; b < NB; ++b) {
-                                float(&a)[4] = acc[2 * rp + q][b];
-                                a[0] = fmaf(sc.x, c[q][b][0], a[0]);
-                                a[1] = fmaf(sc.x, c[q][b][1], a[1]);
-                                a[2] = fmaf(sc.y, c[q][b][2], a[2]);
-                                a[3] = fmaf(sc.y, c[q][b][3], a[3]);
-                            }
+                            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    acc[2 * rp + q][b][e] =
+                                        fmaf(e < 2 ? sc.x : sc.y, c[q][b][e], acc[2 * rp + q][b][e]);
                         }
                     }
                 }
             }
         }
         __syncwarp();  // every lane has read the record before its stage is filled again
-        issue(i + kStages);
+        issue(i + p.stages);
+    }
     }
     cp_async_wait<0>();
     __syncwarp();
 
     // Partial sums [token][row] of each warp over its own ring.
-    float* part = reinterpret_cast<float*>(smem + warp * kStages * p.record_bytes);
+    {
+        float* part = reinterpret_cast<float*>(smem + warp * p.ring_bytes);
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+        for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            float* at = part + (8 * b + 2 * t) * kPartStride + 16 * r + g;
-            at[0] = acc[r][b][0];
-            at[kPartStride] = acc[r][b][1];
-            at[8] = acc[r][b][2];
-            at[kPartStride + 8] = acc[r][b][3];
-        }
-    if (p.cluster > 1) cluster_barrier();
-    else __syncthreads();
-
-    const int tokens = min(8 * NB, p.m - token0);
-    const int64_t row0 = tile * kTileRows;
-    for (int e = rank * kThreads + threadIdx.x; e < tokens * kTileRows; e += kThreads * p.cluster) {
-        const int token = e / kTileRows, row = e % kTileRows;
+            for (int b = 0; b < NB; ++b) {
+                float* at = part + (8 * b + 2 * t) * kPartStride + 16 * r + g;
+                at[0] = acc[r][b][0];
+                at[kPartStride] = acc[r][b][1];
+                at[8] = acc[r][b][2];
+                at[kPartStride + 8] = acc[r][b][3];
+            }
+    }
+    __syncthreads();
+    const int tiles_here = kWarps / p.ksplit;
+    const int outputs = tokens * tiles_here * kTileRows;
+    const auto own_sum = [&](int e, uint32_t* at) {  // of this CTA's ksplit warps
+        const int token = e / (tiles_here * kTileRows), row = e % (tiles_here * kTileRows);
+        *at = mv::smem_addr(smem) + row / kTileRows * p.ksplit * p.ring_bytes +
+              (token * kPartStride + row % kTileRows) * 4;
+        float v = __uint_as_float(lds32(*at));
+        for (int w = 1; w < p.ksplit; ++w) v += __uint_as_float(lds32(*at + w * p.ring_bytes));
+        return v;
+    };
+    if (p.cluster > 1) {
+        if (p.ksplit > 1)
+            for (int e = threadIdx.x; e < outputs; e += kThreads) {
+                uint32_t at;
+                const float v = own_sum(e, &at);
+                asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
+            }
+        cluster_barrier();
+    }
+    const int64_t row0 = tile0 * kTileRows;
+    for (int e = rank * kThreads + threadIdx.x; e < outputs; e += kThreads * p.cluster) {
+        const int token = e / (tiles_here * kTileRows), row = e % (tiles_here * kTileRows);
         if (row0 + row >= p.n) continue;
         float v = 0.0f;
-        for (int c = 0; c < p.cluster; ++c)
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const uint32_t at = mv::smem_addr(smem) + w * kStages * p.record_bytes + (token * kPartStride + row) * 4;
-                v += p.cluster > 1 ? ld_cluster(at, c) : __uint_as_float(lds32(at));
-            }
+        if (p.cluster > 1) {
+            const uint32_t at = mv::smem_addr(smem) + row / kTileRows * p.ksplit * p.ring_bytes +
+                                (token * kPartStride + row % kTileRows) * 4;
+            for (int c = 0; c < p.cluster; ++c) v += ld_cluster(at, c);
+        } else {
+            uint32_t at;
+            v = own_sum(e, &at);
+        }
         const int64_t out_row = token0 + token;
+        v *= ZEROS && KIND == kI8 ? 1.0f : A::kScale;
         if (p.x_scale) v *= p.x_scale[out_row];
         if (p.bias) v += load_as_float(p.bias, row0 + row, p.out_dtype);
         if (p.residual) v += load_as_float(p.residual, out_row * p.residual_stride + row0 + row, p.out_dtype);
@@ -507,8 +601,7 @@ __global__ void __launch_bounds__(kThreads) w4_linear_kernel(const LinearParams 
     if (p.cluster > 1) cluster_barrier();  // no CTA leaves while another reads its shared memory
 }
 
-// W written out, rounded once: a warp per record, a lane's word pairs being
-// eight consecutive columns of a row. Bound by the output's bytes.
+// W written out, rounded once: a warp per record. Bound by the output's bytes.
 template <typename T>
 __global__ void __launch_bounds__(256)
 w4_dequantize_kernel(const uint8_t* records, int64_t total, int chunks, int record_bytes, int group, int has_zeros,
@@ -524,10 +617,16 @@ w4_dequantize_kernel(const uint8_t* records, int64_t total, int chunks, int reco
     const int group_runs = group / 32, groups = kChunk / group;
     for (int h = 0; h < 4; ++h) {
         const int gi = h / group_runs;
-        const int c0 = k0 + 32 * h + 8 * t;
+        // Two lanes trade words, so that each holds eight columns in a row: the
+        // even one both quads of the first half of h, the odd one of the second.
+        const int c0 = k0 + 32 * h + 16 * (t & 1) + 4 * (t & 2);
 #pragma unroll
         for (int rp = 0; rp < 2; ++rp) {
-            const uint4 w = __ldg(reinterpret_cast<const uint4*>(rec) + (h * 2 + rp) * 32 + lane);
+            uint4 w = __ldg(reinterpret_cast<const uint4*>(rec) + (h * 2 + rp) * 32 + lane);
+            const uint32_t got0 = __shfl_xor_sync(0xffffffffu, t & 1 ? w.x : w.y, 1);
+            const uint32_t got1 = __shfl_xor_sync(0xffffffffu, t & 1 ? w.z : w.w, 1);
+            if (t & 1) w.x = got0, w.z = got1;
+            else w.y = got0, w.w = got1;
             const uint2 s = __ldg(reinterpret_cast<const uint2*>(rec + kCodeBytes + gi * 128 + g * 16 + rp * 8));
             uint32_t z = 0;
             if (has_zeros) z = __ldg(reinterpret_cast<const uint32_t*>(rec + kCodeBytes + groups * 128 + gi * 64 + g * 8 + rp * 4));

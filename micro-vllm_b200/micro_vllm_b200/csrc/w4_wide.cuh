@@ -1,0 +1,468 @@
+// Products with 4-bit weights for more tokens than a few: 128 weight rows by NT
+// tokens per CTA on the 5th-generation tensor cores (tcgen05.mma).
+//
+//   D[128, NT] = A[128, group] . X[NT, group]^T    for each group of columns
+//   acc[row, :] += scale[row, group] * D[row, :]
+//
+// A holds code - zero (small integers, exact in 16 bits or int8) in tensor
+// memory: four warps turn the records' words into operand registers by masks,
+// as the mma.sync kernel does, and tcgen05.st.16x256b (int8: 16x128b) puts a
+// lane's registers, rows g and g + 8 and columns 16 e + 4 t + s, in place without
+// passing shared memory. X lies in shared memory (K-major, 128-byte swizzle).
+// Each group's D is its own accumulation, in one of two TMEM buffers; four other
+// warps add it, scaled, to fp32 sums in registers, a thread per weight row.
+//
+// What bounds it: as in the mma.sync kernel the codes' conversion, about 22
+// cycles per 256 weights and scheduler at the copy bandwidth, of which bf16
+// takes 14 of the ALU; the tensor work does not show up to 128 tokens. Weights
+// in TMEM leave shared memory to X alone (A there would be written and read at
+// twice the bandwidth that is left).
+//
+// Warps: 0-7 convert, two sets of four taking chunks in turn (warp w fills lanes
+// 32 (w % 4).. of A); then sets of four that load X (cp.async, three chunks ahead)
+// and drain 32 columns of D each; the last issues the MMAs. A wait that finds its
+// barrier complete still costs some 200 cycles, as does a commit, so there are few
+// of them, and two sets convert so that one's waits hide behind the other. Every
+// wait is bounded (2 s): one that gives up sets the device status, and the CTA's
+// results are NaN.
+#pragma once
+
+#include "w4_linear.cuh"
+
+namespace mvq {
+
+constexpr int kWideRows = 128;
+constexpr int kWideXBuffers = 4;
+constexpr int kWidePartStride = 132;  // floats per token of the partial sums [token][128 rows]
+
+template <int KIND, int NT, int GROUP, bool ZEROS>
+struct WideShape {
+    static constexpr int kGroups = kChunk / GROUP;
+    static constexpr int kCols = NT < 32 ? NT : 32;        // columns of D that a set drains
+    static constexpr int kSets = NT / kCols;
+    static constexpr int kThreads = (8 + 4 * kSets + 1) * 32;
+    static constexpr int kCtas = NT <= 32 ? 2 : 1;         // per SM
+    static constexpr int kStages = NT == 64 ? 5 : 3;       // records in flight per converting warp
+    static constexpr int kACols = KIND == kI8 ? 32 : 64;   // TMEM columns of a chunk of A
+    static constexpr int kABuffers = NT <= 32 && KIND != kI8 ? 3 : 4;
+    static constexpr int kTmemCols = NT <= 32 ? 256 : 512;
+    static_assert(kABuffers * kACols + 2 * NT <= kTmemCols, "TMEM columns");
+    static constexpr int kXBytes = NT * (KIND == kI8 ? 128 : 256);
+    static constexpr int kStageBytes = kCodeBytes / 2 + (ZEROS ? kGroups * 64 : 0);
+    static constexpr int kScaleBytes = kSets * kGroups * 128 * 4;  // per chunk: a word for each draining thread
+    static constexpr int kRings = 8 * kStages * kStageBytes;
+    static constexpr int kUsed = kWideXBuffers * (kXBytes + kScaleBytes) + kRings;
+    static constexpr int kPart = NT * kWidePartStride * 4;
+    static constexpr int kSmem = (kUsed > kPart ? kUsed : kPart) + 1024;
+};
+
+__device__ __forceinline__ uint64_t sw128_desc(uint32_t addr) {
+    return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | (static_cast<uint64_t>(1) << 16) |
+           (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) |
+           (static_cast<uint64_t>(2) << 61);
+}
+
+__device__ __forceinline__ bool elect_one() {
+    uint32_t leader;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(leader));
+    return leader != 0;
+}
+
+// D fp32 (1) or s32 (2); A and B fp16 (0), bf16 (1) or s8 (1); both K-major.
+template <int KIND, int NT>
+__host__ __device__ constexpr uint32_t wide_idesc() {
+    return ((KIND == kI8 ? 2u : 1u) << 4) | ((KIND == kF16 ? 0u : 1u) << 7) | ((KIND == kF16 ? 0u : 1u) << 10) |
+           (static_cast<uint32_t>(NT >> 3) << 17) | (static_cast<uint32_t>(kWideRows >> 4) << 24);
+}
+
+template <int KIND>
+__device__ __forceinline__ void wide_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+    if constexpr (KIND == kI8)
+        asm volatile(
+            "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+            " tcgen05.mma.cta_group::1.kind::i8 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+            "r"(a), "l"(b), "r"(idesc), "r"(add));
+    else
+        asm volatile(
+            "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+            " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+            "r"(a), "l"(b), "r"(idesc), "r"(add));
+}
+
+__device__ __forceinline__ void wide_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void wide_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 16 rows x 16 32-bit columns: lane (g, t) holds columns 8 j + 2 t, + 1 of row g (r[4 j], r[4 j + 1]) and of row g + 8.
+__device__ __forceinline__ void tmem_st_16x16(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.16x256b.x2.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+// 16 rows x 8 columns: lane (g, t) holds columns t (r[0]) and 4 + t (r[2]) of row g, r[1] and r[3] of row g + 8.
+__device__ __forceinline__ void tmem_st_16x8(uint32_t taddr, const uint32_t (&r)[4]) {
+    asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ld_16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+
+__device__ __forceinline__ void cp_async_16_or_zero(uint32_t dst, const void* src, bool real) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+
+template <int KIND, int NT, int GROUP, bool ZEROS>
+__global__ void __launch_bounds__(WideShape<KIND, NT, GROUP, ZEROS>::kThreads, WideShape<KIND, NT, GROUP, ZEROS>::kCtas)
+w4_wide_kernel(const LinearParams p) {
+    using A = Act<KIND>;
+    using Shape = WideShape<KIND, NT, GROUP, ZEROS>;
+    constexpr int kGroups = Shape::kGroups;
+    constexpr int kRecord = record_size(GROUP, ZEROS);
+    constexpr int kStages = Shape::kStages, kAB = Shape::kABuffers, kSets = Shape::kSets;
+    constexpr int kMmaWarp = 8 + 4 * kSets;
+    extern __shared__ uint8_t smem_raw[];
+    // Per chunk one barrier for both operands (full) and one for the end of its
+    // last group (done, which frees A and X and hands over D); part_done and
+    // d_empty only serve chunks of several groups.
+    __shared__ __align__(8) uint64_t full[kAB], done[kAB], part_done[2], d_empty[2], drained;
+    __shared__ uint32_t s_tmem;
+    __shared__ volatile int s_failed;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = p.cluster > 1 ? static_cast<int>(cluster_rank()) : 0;
+    const int64_t block = static_cast<int64_t>(blockIdx.x) / p.cluster;  // of 128 weight rows
+    const int token0 = blockIdx.y * NT;
+    const int tokens = min(NT, p.m - token0);
+    const int begin = static_cast<int>(static_cast<int64_t>(p.chunks) * rank / p.cluster);
+    const int n = static_cast<int>(static_cast<int64_t>(p.chunks) * (rank + 1) / p.cluster) - begin;
+
+    uint8_t* const smem =
+        reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    const uint32_t xs = mv::smem_addr(smem);
+    const uint32_t scale_at = xs + kWideXBuffers * Shape::kXBytes;
+    const uint32_t rings = scale_at + kWideXBuffers * Shape::kScaleBytes;
+
+    // A converting or draining warp w has rows 32 (w % 4).. of the 128: half p = w & 1
+    // of tile (w % 4) >> 1. A second tile beyond the weight's last reads the
+    // last one; its rows are never stored.
+    const int quarter = warp & 3;
+    const int64_t tile = min(2 * block + (quarter >> 1), static_cast<int64_t>(p.tiles) - 1);
+    const uint8_t* const records = p.records + (tile * p.chunks + begin) * static_cast<int64_t>(kRecord);
+    const uint8_t* const codes = records + (quarter & 1) * 512 + lane * 16;
+    const uint32_t ring = rings + (warp & 7) * kStages * Shape::kStageBytes;
+    const int set = warp < 8 ? warp >> 2 : (warp - 8) >> 2;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kAB; ++i) {
+            mv::mbar_init(mv::smem_addr(&full[i]), 4 + 4 * kSets);  // a converting set and all loading warps
+            mv::mbar_init(mv::smem_addr(&done[i]), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mv::mbar_init(mv::smem_addr(&part_done[i]), 1);
+            mv::mbar_init(mv::smem_addr(&d_empty[i]), 4 * kSets);
+        }
+        mv::mbar_init(mv::smem_addr(&drained), 1);
+        s_failed = 0;
+        mv::fence_mbar_init();
+    }
+    if (warp < 8)  // into L2 only: what the grid before wrote is not visible yet
+        for (int i = set; i < 2 * kStages && i < n; i += 2)
+            if (lane * 128 < kRecord)
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(records + static_cast<int64_t>(i) * kRecord + lane * 128));
+    mv::wait_for_prior_grid();
+    mv::allow_next_grid();
+
+    int fill = 0;  // stage of the ring that the next record goes to
+    const auto issue_codes = [&](int i) {
+        if (i < n) {
+            const uint8_t* rec = codes + static_cast<int64_t>(i) * kRecord;
+            const uint32_t dst = ring + fill * Shape::kStageBytes + lane * 16;
+#pragma unroll
+            for (int h = 0; h < 4; ++h) cp_async_16(dst + h * 512, rec + h * 1024);
+            if (ZEROS && lane < kGroups * 4)
+                cp_async_16(dst + kCodeBytes / 2, records + static_cast<int64_t>(i) * kRecord + kCodeBytes +
+                                                      kGroups * 128 + lane * 16);
+        }
+        cp_async_commit();
+        fill = fill + 1 == kStages ? 0 : fill + 1;
+    };
+    if (warp < 8)
+        for (int i = 0; i < kStages; ++i) issue_codes(set + 2 * i);
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(mv::smem_addr(&s_tmem)),
+                     "r"(Shape::kTmemCols));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = s_tmem;
+    const uint32_t d_col = tmem + kAB * Shape::kACols;
+    const auto wait = [&](uint64_t* bar, int parity) {  // of a whole warp
+        const bool ok = __all_sync(0xffffffffu, mv::mbar_wait_bounded(mv::smem_addr(bar), parity & 1));
+        if (!ok) {
+            s_failed = 1;
+            if (lane == 0) atomicOr(&mv::g_device_status, mv::kStatusWaitTimeout);
+        }
+        return ok;
+    };
+
+    if (warp < 8) {
+        const int g = lane >> 2;
+        int drain = 0;
+        const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+        for (int i = set; i < n; i += 2) {
+            cp_async_wait<kStages - 1>();
+            if (ZEROS) __syncwarp();
+            const uint32_t rec = ring + drain * Shape::kStageBytes;
+            drain = drain + 1 == kStages ? 0 : drain + 1;
+            if (i >= kAB && !wait(&done[i % kAB], i / kAB - 1)) break;
+            fence_after();
+            const uint32_t a_col = lanes + (i % kAB) * Shape::kACols;
+            uint32_t zl[2], zh[2];
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+                if (h % (GROUP / 32) == 0) {
+                    uint32_t z = 0;
+                    if (ZEROS) z = lds32(rec + kCodeBytes / 2 + (h / (GROUP / 32)) * 64 + g * 8 + (quarter & 1) * 4);
+                    if constexpr (KIND == kI8) {
+                        const uint32_t u = (z ^ 0x88888888u) & 0x0f0f0f0fu;
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            zl[q] = __byte_perm(u, 0, q ? 0x2222 : 0x0000);
+                            zh[q] = __byte_perm(u, 0, q ? 0x3333 : 0x1111);
+                        }
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            zl[q] = A::zero_low(8 + static_cast<int8_t>(z >> (16 * q)));
+                            zh[q] = A::zero_high(8 + static_cast<int8_t>(z >> (16 * q + 8)));
+                        }
+                    }
+                }
+                const uint4 w = lds128(rec + h * 512 + lane * 16);
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const uint32_t w0 = q ? w.z : w.x, w1 = q ? w.w : w.y;
+                    const uint32_t at = a_col + (static_cast<uint32_t>(q * 16) << 16);
+                    if constexpr (KIND == kI8) {
+                        // 32 columns of h: bytes in the columns' order (the codes' is 0, 2, 1, 3).
+                        uint32_t r[4];
+                        if (ZEROS) {
+                            r[0] = bytes_minus(w0, zl[q]), r[1] = bytes_minus(w0 >> 4, zh[q]);
+                            r[2] = bytes_minus(w1, zl[q]), r[3] = bytes_minus(w1 >> 4, zh[q]);
+                        } else {
+                            r[0] = (w0 << 4) & 0xf0f0f0f0u, r[1] = w0 & 0xf0f0f0f0u;
+                            r[2] = (w1 << 4) & 0xf0f0f0f0u, r[3] = w1 & 0xf0f0f0f0u;
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) r[e] = __byte_perm(r[e], 0, 0x3120);
+                        tmem_st_16x8(at + h * 8, r);
+                    } else {
+                        uint32_t a0[4], a1[4];
+                        A::weights(w0, zl[q], zh[q], a0);
+                        A::weights(w1, zl[q], zh[q], a1);
+                        const uint32_t r[8] = {a0[0], a0[2], a0[1], a0[3], a1[0], a1[2], a1[1], a1[3]};
+                        tmem_st_16x16(at + h * 16, r);
+                    }
+                }
+            }
+            if (ZEROS) __syncwarp();
+            issue_codes(i + 2 * kStages);
+            wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) wide_arrive(mv::smem_addr(&full[i % kAB]));
+        }
+        cp_async_wait<0>();
+    } else if (warp == kMmaWarp) {
+        // The whole warp runs the loop, so that the operands' addresses are
+        // uniform; one elected lane issues.
+        constexpr int kSteps = KIND == kI8 ? GROUP / 32 : GROUP / 16;  // MMAs per group
+        const bool leader = elect_one();
+        bool ok = true;
+        for (int i = 0; i < n && ok; ++i) {
+            ok = wait(&full[i % kAB], i / kAB);
+#pragma unroll
+            for (int gi = 0; gi < kGroups; ++gi) {
+                const int u = i * kGroups + gi;
+                // With one group the loading warps' arrival for chunk i says that D of chunk i - 2 is drained.
+                if (kGroups > 1 && u >= 2) ok = ok && wait(&d_empty[u & 1], (u >> 1) - 1);
+                fence_after();
+                if (leader && ok) {
+                    const uint32_t a_at = tmem + (i % kAB) * Shape::kACols + gi * kSteps * 8;
+                    const uint32_t x_at = xs + (i % kWideXBuffers) * Shape::kXBytes;
+#pragma unroll
+                    for (int s = 0; s < kSteps; ++s) {
+                        const int step = gi * kSteps + s;
+                        const uint32_t b = KIND == kI8 ? x_at + step * 32 : x_at + (step >> 2) * (NT * 128) + (step & 3) * 32;
+                        wide_mma<KIND>(d_col + (u & 1) * NT, a_at + s * 8, sw128_desc(b), wide_idesc<KIND, NT>(), s > 0);
+                    }
+                    wide_commit(mv::smem_addr(gi == kGroups - 1 ? &done[i % kAB] : &part_done[(i * (kGroups - 1) + gi) & 1]));
+                }
+                __syncwarp();
+            }
+        }
+        // Everything issued completes before TMEM is freed.
+        if (leader) wide_commit(mv::smem_addr(&drained));
+        __syncwarp();
+        wait(&drained, 0);
+    } else {
+        constexpr int kLoaders = 128 * kSets;
+        const int lt = threadIdx.x - 256;
+        constexpr int kUnits = KIND == kI8 ? 8 : 16;  // 16-byte units of a token's chunk
+        constexpr int kTurns = NT * kUnits / kLoaders;
+        constexpr int kTokens = kLoaders / kUnits;    // tokens of a turn
+        const int x_size = p.x_dtype == kF32 ? 4 : p.x_dtype >= kI8 ? 1 : 2;
+        // This thread's scale: row `lane` of the quarter, its pair of rows g and g + 8 in a word.
+        const uint8_t* const scale = records + kCodeBytes + ((lane & 7) * 8 + (quarter & 1) * 4 + (lane >> 4) * 2) * 2;
+        // This thread's units: `unit` of tokens first, first + kTokens, ... (all at one place of the swizzle).
+        const int first = lt / kUnits, unit = lt % kUnits;
+        const uint32_t unit_at = (unit >> 3) * (NT * 128) + first * 128 + (((unit & 7) ^ (first & 7)) << 4);
+        const uint8_t* const rows = static_cast<const uint8_t*>(p.x) + (token0 + first) * p.x_stride * x_size;
+        const int64_t row_step = kTokens * p.x_stride * x_size;
+        const auto issue_x = [&](int i) {
+            if (lane < kGroups && i + 2 < n)  // the scales come from memory: into L2 before they are copied
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(records + static_cast<int64_t>(i + 2) * kRecord + kCodeBytes + lane * 128));
+            if (i < n) {
+                const uint32_t dst = xs + (i % kWideXBuffers) * Shape::kXBytes + unit_at;
+                const int k = (begin + i) * kChunk + unit * (KIND == kI8 ? 16 : 8);
+                if (p.x_units) {
+#pragma unroll
+                    for (int j = 0; j < kTurns; ++j) {
+                        const bool real = first + j * kTokens < tokens && k < p.k;
+                        cp_async_16_or_zero(dst + j * kTokens * 128,
+                                            real ? rows + j * row_step + k * x_size : static_cast<const uint8_t*>(p.x), real);
+                    }
+                } else {  // a loop, and apart from the other: what warps of several roles run has to fit the instruction cache
+#pragma unroll 1
+                    for (int j = 0; j < kTurns; ++j) {
+                        const int limit = first + j * kTokens < tokens ? p.k : 0;
+                        uint32_t r[1][A::kRunBytes / 4];
+                        uint4 v;
+                        load_run<KIND>(p, rows + j * row_step, k, limit, r);
+                        if constexpr (KIND == kI8) {
+                            v.x = r[0][0], v.y = r[0][1];
+                            load_run<KIND>(p, rows + j * row_step, k + 8, limit, r);
+                            v.z = r[0][0], v.w = r[0][1];
+                        } else {
+                            v = make_uint4(r[0][0], r[0][1], r[0][2], r[0][3]);
+                        }
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + j * kTokens * 128),
+                                     "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                                     : "memory");
+                    }
+                }
+#pragma unroll
+                for (int gi = 0; gi < kGroups; ++gi)
+                    cp_async_4(scale_at + (i % kWideXBuffers) * Shape::kScaleBytes + (gi * kLoaders + lt) * 4,
+                               scale + static_cast<int64_t>(i) * kRecord + gi * 128);
+            }
+            cp_async_commit();
+        };
+        float acc[Shape::kCols];
+#pragma unroll
+        for (int e = 0; e < Shape::kCols; ++e) acc[e] = 0.0f;
+        const uint32_t lanes = d_col + set * Shape::kCols + (static_cast<uint32_t>(quarter * 32) << 16);
+        const auto publish = [&](int i) {  // chunk i of X is in shared memory, D of chunk i - 2 in registers
+            if (i >= n) return;
+            mv::fence_proxy_async_smem();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) wide_arrive(mv::smem_addr(&full[i % kAB]));
+        };
+        for (int i = 0; i < kWideXBuffers - 1; ++i) issue_x(i);
+        cp_async_wait<kWideXBuffers - 2>();
+        publish(0);
+        bool ok = true;
+        for (int i = 0; i < n && ok; ++i) {
+#pragma unroll
+            for (int gi = 0; gi < kGroups; ++gi) {
+                if (gi == 0) {
+                    // Chunk i + kWideXBuffers - 1 goes where chunk i - 1 was, whose D this warp has drained.
+                    issue_x(i + kWideXBuffers - 1);
+                    cp_async_wait<kWideXBuffers - 2>();
+                    publish(i + 1);
+                }
+                const int u = i * kGroups + gi, v = i * (kGroups - 1) + gi;
+                const uint32_t pair = lds32(scale_at + (i % kWideXBuffers) * Shape::kScaleBytes + (gi * kLoaders + lt) * 4);
+                const float2 both = scale_pair(pair, p.scale_bf16);
+                const float sc = lane & 8 ? both.y : both.x;
+                ok = ok && (gi == kGroups - 1 ? wait(&done[i % kAB], i / kAB) : wait(&part_done[v & 1], v >> 1));
+                if (!ok) break;
+                fence_after();
+                const uint32_t from = lanes + (u & 1) * NT;
+#pragma unroll
+                for (int c = 0; c < Shape::kCols; c += 16) {
+                    uint32_t r[16];
+                    tmem_ld_16(from + c, r);
+                    wait_ld();
+                    if (kGroups > 1 && c + 16 == Shape::kCols) {
+                        fence_before();
+                        __syncwarp();
+                        if (lane == 0) wide_arrive(mv::smem_addr(&d_empty[u & 1]));
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        // s32 to fp32: 1.5 2^23's bits plus the sum (below 2^22) are the float 1.5 2^23 + sum.
+                        const float f = KIND == kI8 ? __uint_as_float(r[e] + 0x4b400000u) - 12582912.0f
+                                                    : __uint_as_float(r[e]);
+                        acc[c + e] = fmaf(sc, f, acc[c + e]);
+                    }
+                }
+            }
+        }
+        cp_async_wait<0>();
+        // The last group's D is complete, so no MMA reads X and no warp converts
+        // any more, and behind this barrier no warp reads a scale: the partial
+        // sums go over them.
+        asm volatile("bar.sync 1, %0;" ::"n"(kLoaders) : "memory");
+        float* part = reinterpret_cast<float*>(smem) + set * Shape::kCols * kWidePartStride + quarter * 32 + lane;
+        const float poison = ok && !s_failed ? 0.0f : __int_as_float(0x7fffffff);
+#pragma unroll
+        for (int e = 0; e < Shape::kCols; ++e) part[e * kWidePartStride] = acc[e] + poison;
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == kMmaWarp) {  // before any wait for another CTA: none may wait for this one's columns meanwhile
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Shape::kTmemCols));
+    }
+    if (p.cluster > 1) cluster_barrier();
+    const int64_t row0 = block * kWideRows;
+    for (int e = rank * Shape::kThreads + threadIdx.x; e < tokens * kWideRows; e += Shape::kThreads * p.cluster) {
+        const int token = e / kWideRows, row = e % kWideRows;
+        if (row0 + row >= p.n) continue;
+        const uint32_t at = xs + (token * kWidePartStride + row) * 4;
+        float v = 0.0f;
+        if (p.cluster > 1)
+            for (int c = 0; c < p.cluster; ++c) v += ld_cluster(at, c);
+        else
+            v = __uint_as_float(lds32(at));
+        const int64_t out_row = token0 + token;
+        v *= ZEROS && KIND == kI8 ? 1.0f : A::kScale;
+        if (p.x_scale) v *= p.x_scale[out_row];
+        if (p.bias) v += load_as_float(p.bias, row0 + row, p.out_dtype);
+        if (p.residual) v += load_as_float(p.residual, out_row * p.residual_stride + row0 + row, p.out_dtype);
+        store_from_float(p.out, out_row * p.out_stride + row0 + row, p.out_dtype, v);
+    }
+    if (p.cluster > 1) cluster_barrier();  // no CTA leaves while another reads its shared memory
+}
+
+}  // namespace mvq

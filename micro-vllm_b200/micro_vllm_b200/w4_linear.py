@@ -93,12 +93,12 @@ def pack_w4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | Non
     tiles, chunks, per_chunk = -(-n // TILE_ROWS), -(-k // CHUNK), CHUNK // group_size
     pad = torch.nn.functional.pad
     rows = tiles * TILE_ROWS - n
-    # [tile, p, q, half, g, chunk, h, t, e, s]: row 32p + 16q + 8half + g, column 32h + 8t + 4e + s. Codes are
+    # [tile, p, q, half, g, chunk, h, e, t, s]: row 32p + 16q + 8half + g, column 32h + 16e + 4t + s. Codes are
     # stored with their highest bit inverted (code - 8 in two's complement); columns beyond K hold code 8.
     c = pad(codes, (0, chunks * CHUNK - k, 0, rows), value=8).bitwise_xor_(8)
-    c = c.view(tiles, 2, 2, 2, 8, chunks, 4, 4, 2, 4)
-    c = c[:, :, :, 0] | (c[:, :, :, 1] << 4)                # [tile, p, q, g, chunk, h, t, e, s]
-    c = c.permute(0, 4, 5, 1, 3, 6, 2, 7, 8)[..., [0, 2, 1, 3]].reshape(tiles, chunks, TILE_ROWS * CHUNK // 2)
+    c = c.view(tiles, 2, 2, 2, 8, chunks, 4, 2, 4, 4)
+    c = c[:, :, :, 0] | (c[:, :, :, 1] << 4)                # [tile, p, q, g, chunk, h, e, t, s]
+    c = c.permute(0, 4, 5, 1, 3, 7, 2, 6, 8)[..., [0, 2, 1, 3]].reshape(tiles, chunks, TILE_ROWS * CHUNK // 2)
 
     def by_group(values):  # [tile, chunk, bytes of the chunk's groups]
         values = pad(values, (0, chunks * per_chunk - groups, 0, rows))

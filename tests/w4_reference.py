@@ -49,7 +49,7 @@ def unpack_records(weight):
                             at = (((h * 2 + p) * 32 + lane) * 4 + word) * 4
                             for byte, s in enumerate((0, 2, 1, 3)):
                                 value = int(record[at + byte])
-                                column = j * 128 + 32 * h + 8 * t + 4 * e + s
+                                column = j * 128 + 32 * h + 16 * e + 4 * t + s
                                 row = i * 64 + 32 * p + 16 * q + g
                                 codes[row, column] = (value & 15) ^ 8
                                 codes[row + 8, column] = (value >> 4) ^ 8
