@@ -63,21 +63,44 @@ def silu_mul(gate_up: torch.Tensor, out: torch.Tensor | None = None) -> torch.Te
     return out
 
 
-def _no_grad(*tensors):
-    _check(not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors),
-           'row operations do not support gradients')
+_strided = torch.strided
+_grad_enabled = torch.is_grad_enabled
 
 
-def _output_rows(t, shape, dtype, device, name):
-    """A given output, checked, as [rows, width]."""
-    _check(isinstance(t, torch.Tensor) and t.shape == shape and t.dtype == dtype and t.device == device,
-           f'{name} must have the shape {tuple(shape)}, dtype {dtype} and the device of the input')
-    _no_grad(t)
-    _check(t.dim() == 2 or t.is_contiguous(), f'{name}: tensors other than [rows, width] must be contiguous')
-    flat = t if t.dim() == 2 else t.view(-1, shape[-1])
-    _check(shape[-1] == 1 or flat.stride(1) == 1, f'{name} requires feature stride 1')
-    _check(flat.shape[0] <= 1 or flat.stride(0) >= shape[-1], f'rows of {name} must not overlap')
-    return flat
+def _input_rows(t, shape, dtype, index, name):
+    """Row stride of an input [..., width] of this shape, dtype and device, seen as [rows, width]."""
+    if not (t.is_cuda and t.get_device() == index and t.dtype is dtype and t.shape == shape and t.layout is _strided
+            and not t.is_neg()):
+        _check(False, f'{name} must match the input: a strided CUDA tensor of its shape, dtype and device')
+    if t.requires_grad and _grad_enabled():
+        _check(False, 'row operations do not support gradients')
+    if t.is_contiguous():
+        return shape[-1]
+    if len(shape) == 2:
+        row, feature = t.stride()
+        _check(feature == 1 or shape[1] == 1, f'{name} requires feature stride 1')
+        _check(shape[0] <= 1 or row >= shape[1], f'rows of {name} must not overlap')
+        return row
+    return _check(False, f'{name}: tensors other than [rows, width] must be contiguous')
+
+
+def _fresh(like, shape, dtype):
+    """An uninitialised contiguous tensor (`like`, where it has the shape, is the cheaper way to say so)."""
+    if like.is_contiguous():
+        return torch.empty_like(like, dtype=dtype)
+    return torch.empty(shape, dtype=dtype, device=like.device)
+
+
+def _fresh_scales(shape, device):
+    if len(shape) == 2:
+        return torch.empty(shape[0], dtype=torch.float32, device=device)
+    return torch.empty(shape[:-1], dtype=torch.float32, device=device)
+
+
+def _check_scales(scales, shape, index):
+    _check(scales.is_cuda and scales.shape == shape and scales.dtype == torch.float32 and scales.is_contiguous()
+           and scales.get_device() == index and not (scales.requires_grad and _grad_enabled()),
+           'scales must be contiguous float32, one per row, on the device of the input')
 
 
 def _disjoint(out, others, same=()):
@@ -91,55 +114,63 @@ def _disjoint(out, others, same=()):
 
 
 def _launch(entry, packed, index):
-    stream = current_stream_raw(index)
+    """Enqueue on the current stream of device `index`, with that device current."""
     if torch.cuda.current_device() == index:
-        return _quant_native.check(entry(packed, stream))
-    with torch.cuda.device(index):
-        return _quant_native.check(entry(packed, stream))
+        status = entry(packed, current_stream_raw(index))
+    else:
+        with torch.cuda.device(index):
+            status = entry(packed, current_stream_raw(index))
+    if status:
+        _quant_native.check(status)
 
 
 def _add_rms_norm(x, residual, weight, eps, out, out_dtype, scales, residual_out):
-    rows = _rows(x)
-    hidden, device = x.shape[-1], x.device
-    _check(rows.shape[1] > 0, 'rows must not be empty')
-    _check(weight.shape == (hidden,) and weight.dtype == x.dtype and weight.is_contiguous()
-           and weight.device == device, 'weight must be a contiguous [hidden] tensor of the input dtype')
-    _no_grad(x, residual, weight)
+    dtype, shape = x.dtype, x.shape
+    code = DTYPE_CODES.get(dtype)
+    _check(x.is_cuda and code is not None and shape, 'row operations take CUDA float tensors')
+    index, device, hidden = x.get_device(), x.device, shape[-1]
+    _check(hidden > 0, 'rows must not be empty')
+    x_stride = _input_rows(x, shape, dtype, index, 'x')
+    if weight.shape != (hidden,) or weight.dtype is not dtype or not weight.is_contiguous() or \
+            weight.get_device() != index:
+        _check(False, 'weight must be a contiguous [hidden] tensor of the input dtype')
+    _check(not (weight.requires_grad and _grad_enabled()), 'row operations do not support gradients')
     residual_at = residual_stride = sum_at = sum_stride = scales_at = 0
+    given_out, given_sum = out is not None, residual_out is not None
     if residual is not None:
-        _check(residual.shape == x.shape and residual.dtype == x.dtype and residual.device == device,
-               'residual must match x')
-        flat = _rows(residual)
-        residual_at, residual_stride = flat.data_ptr(), flat.stride(0)
-        fresh = residual_out is None
-        if fresh:
-            residual_out = torch.empty(x.shape, dtype=x.dtype, device=device)
-        flat = _output_rows(residual_out, x.shape, x.dtype, device, 'residual_out')
-        if not fresh:
+        residual_stride = _input_rows(residual, shape, dtype, index, 'residual')
+        residual_at = residual.data_ptr()
+        if given_sum:
+            sum_stride = _input_rows(residual_out, shape, dtype, index, 'residual_out')
             _disjoint(residual_out, (x, residual, weight), same=(x, residual))
-        sum_at, sum_stride = flat.data_ptr(), flat.stride(0)
-    else:
-        _check(residual_out is None, 'residual_out needs a residual')
-    fresh = out is None
-    if fresh:
-        out = torch.empty(x.shape, dtype=out_dtype, device=device)
-    flat = _output_rows(out, x.shape, out_dtype, device, 'out')
-    if not fresh:
-        _disjoint(out, (x, residual, weight, residual_out), same=(x,) if residual_out is not x else ())
-    if out_dtype in QUANT_CODES:
-        if scales is None:
-            scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=device)
         else:
-            _check(scales.shape == x.shape[:-1] and scales.dtype == torch.float32 and scales.is_contiguous()
-                   and scales.device == device, 'scales must be contiguous float32, one per row')
-            _disjoint(scales, (x, residual, weight, out, residual_out))
+            residual_out, sum_stride = _fresh(x, shape, dtype), hidden
+        sum_at = residual_out.data_ptr()
+    else:
+        _check(not given_sum, 'residual_out needs a residual')
+        residual_out = x
+    if given_out:
+        out_stride = _input_rows(out, shape, out_dtype, index, 'out')
+        _disjoint(out, (x, residual, weight, residual_out if residual is not None else None),
+                  same=(x,) if residual is None or residual_out is not x else ())
+    else:
+        out, out_stride = _fresh(x, shape, out_dtype), hidden
+    out_code = QUANT_CODES.get(out_dtype)
+    if out_code is None:
+        out_code = code
+    elif scales is None:
+        scales = _fresh_scales(shape, device)
         scales_at = scales.data_ptr()
-    if rows.shape[0]:
+    else:
+        _check_scales(scales, shape[:-1], index)
+        _disjoint(scales, (x, residual, weight, out, residual_out))
+        scales_at = scales.data_ptr()
+    rows = x.numel() // hidden
+    if rows:
         _launch(_quant_native.library().mvq_add_rms_norm, _quant_native.pack_norm(
-            rows.data_ptr(), rows.stride(0), residual_at, residual_stride, weight.data_ptr(), flat.data_ptr(),
-            flat.stride(0), scales_at, sum_at, sum_stride, rows.shape[0], hidden, float(eps), DTYPE_CODES[x.dtype],
-            QUANT_CODES[out_dtype] if out_dtype in QUANT_CODES else DTYPE_CODES[out_dtype]), device.index)
-    return out, scales, x if residual is None else residual_out
+            x.data_ptr(), x_stride, residual_at, residual_stride, weight.data_ptr(), out.data_ptr(), out_stride,
+            scales_at, sum_at, sum_stride, rows, hidden, eps, code, out_code), index)
+    return out, scales, residual_out
 
 
 def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float, *,
@@ -175,26 +206,29 @@ def silu_mul_quant(gate_up: torch.Tensor, *, quant_dtype: torch.dtype = torch.in
 
     The product stays in fp32 until its one rounding (``silu_mul`` rounds each step).
     """
-    _check(quant_dtype in QUANT_CODES, 'quant_dtype must be int8 or float8_e4m3fn')
-    rows = _rows(gate_up)
-    _check(rows.shape[1] % 2 == 0 and rows.shape[1] > 0, 'the last dimension must hold gate and up halves')
-    _no_grad(gate_up)
-    width, device = rows.shape[1] // 2, gate_up.device
-    shape = gate_up.shape[:-1] + (width,)
-    fresh = out is None
-    if fresh:
-        out = torch.empty(shape, dtype=quant_dtype, device=device)
-    flat = _output_rows(out, shape, quant_dtype, device, 'out')
-    if not fresh:
+    out_code = QUANT_CODES.get(quant_dtype)
+    _check(out_code is not None, 'quant_dtype must be int8 or float8_e4m3fn')
+    dtype, shape = gate_up.dtype, gate_up.shape
+    code = DTYPE_CODES.get(dtype)
+    _check(gate_up.is_cuda and code is not None and shape, 'row operations take CUDA float tensors')
+    index, device, width = gate_up.get_device(), gate_up.device, shape[-1] // 2
+    _check(shape[-1] % 2 == 0 and width > 0, 'the last dimension must hold gate and up halves')
+    stride = _input_rows(gate_up, shape, dtype, index, 'gate_up')
+    out_shape = shape[:-1] + (width,)
+    if out is None:
+        out = (torch.empty(shape[0], width, dtype=quant_dtype, device=device) if len(shape) == 2
+               else torch.empty(out_shape, dtype=quant_dtype, device=device))
+        out_stride = width
+    else:
+        out_stride = _input_rows(out, out_shape, quant_dtype, index, 'out')
         _disjoint(out, (gate_up,))
     if scales is None:
-        scales = torch.empty(gate_up.shape[:-1], dtype=torch.float32, device=device)
+        scales = _fresh_scales(shape, device)
     else:
-        _check(scales.shape == gate_up.shape[:-1] and scales.dtype == torch.float32 and scales.is_contiguous()
-               and scales.device == device, 'scales must be contiguous float32, one per row')
+        _check_scales(scales, shape[:-1], index)
         _disjoint(scales, (gate_up, out))
-    if rows.shape[0]:
+    rows = gate_up.numel() // (2 * width)
+    if rows:
         _launch(_quant_native.library().mvq_silu_mul_quant, _quant_native.pack_silu(
-            rows.data_ptr(), rows.stride(0), flat.data_ptr(), flat.stride(0), scales.data_ptr(), rows.shape[0], width,
-            DTYPE_CODES[gate_up.dtype], QUANT_CODES[quant_dtype]), device.index)
+            gate_up.data_ptr(), stride, out.data_ptr(), out_stride, scales.data_ptr(), rows, width, code, out_code), index)
     return out, scales

@@ -39,7 +39,7 @@ def _check(condition, message):
 class W4Weight:
     """A [N, K] weight in 4-bit codes, laid out for the kernels (include/mvquant.h). Immutable."""
 
-    __slots__ = ('records', 'shape', 'group_size', 'has_zeros', 'scale_dtype', '_fixed')
+    __slots__ = ('records', 'shape', 'group_size', 'has_zeros', 'scale_dtype', 'index', 'fixed')
 
     def __init__(self, records, shape, group_size, has_zeros, scale_dtype):
         self.records = records
@@ -47,7 +47,9 @@ class W4Weight:
         self.group_size = group_size
         self.has_zeros = has_zeros
         self.scale_dtype = scale_dtype
-        self._fixed = (records.data_ptr(), *self.shape, group_size, int(has_zeros), SCALE_CODES[scale_dtype])
+        self.index = records.get_device()  # -1 on the CPU
+        # The weight's fields of the calls' argument structs.
+        self.fixed = (records.data_ptr(), *self.shape, group_size, int(has_zeros), SCALE_CODES[scale_dtype])
 
     @property
     def device(self):
@@ -145,29 +147,41 @@ def quantize_w4(weight: torch.Tensor, *, group_size: int = 128, zeros: bool = Fa
                    group_size=group_size)
 
 
-def _plain(t, name):
-    _check(t.is_cuda and t.layout == torch.strided and not t.is_neg(), f'{name} must be a strided CUDA tensor')
-    _check(not t.requires_grad or not torch.is_grad_enabled(), f'{name}: 4-bit layers do not support gradients')
+_strided = torch.strided
+_grad_enabled = torch.is_grad_enabled
 
 
-def _flat_rows(t, width, name):
-    """t as [rows, width] without copying."""
-    _check(t.dim() >= 1 and t.shape[-1] == width, f'{name} must have {width} features')
-    if t.dim() == 2:
-        rows = t
-    else:
-        _check(t.is_contiguous(), f'{name}: tensors other than [rows, width] must be contiguous')
-        rows = t.view(-1, width)
-    _check(width == 1 or rows.stride(1) == 1, f'{name} requires feature stride 1')
-    return rows
+def _usable(t, index):
+    """A strided tensor on CUDA device `index` that asks for no gradient."""
+    return (t.is_cuda and t.get_device() == index and t.layout is _strided and not t.is_neg()
+            and not (t.requires_grad and _grad_enabled()))
+
+
+def _refuse(t, name, index):
+    _check(t.is_cuda and t.layout is _strided and not t.is_neg(), f'{name} must be a strided CUDA tensor')
+    _check(not t.requires_grad or not _grad_enabled(), f'{name}: 4-bit layers do not support gradients')
+    _check(t.get_device() == index, f'{name} must be on the device of x')
+
+
+def _row_stride(t, width, name):
+    """Row stride of t [..., width] seen as [rows, width] without copying."""
+    if t.is_contiguous():
+        return width
+    _check(t.dim() == 2, f'{name}: tensors other than [rows, width] must be contiguous')
+    row, feature = t.stride()
+    _check(feature == 1 or width == 1, f'{name} requires feature stride 1')
+    return row
 
 
 def _launch(entry, packed, index):
-    stream = current_stream_raw(index)
+    """Enqueue on the current stream of device `index`, with that device current."""
     if torch.cuda.current_device() == index:
-        return _native.check(entry(packed, stream))
-    with torch.cuda.device(index):
-        return _native.check(entry(packed, stream))
+        status = entry(packed, current_stream_raw(index))
+    else:
+        with torch.cuda.device(index):
+            status = entry(packed, current_stream_raw(index))
+    if status:
+        _native.check(status)
 
 
 def w4_linear(x: torch.Tensor, weight: W4Weight, bias: torch.Tensor | None = None,
@@ -180,63 +194,73 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, bias: torch.Tensor | None = Non
     integers within a group for int8) and rounded once, to ``out_dtype``: the
     type of ``out`` or of the residual or bias, else x's own; 8-bit x needs one
     of these. bias [N] and residual [..., N] have that type; out may be residual.
-    Any number of rows; made for up to 64. Runs on the current stream.
+    Any number of rows; made for a decode step's (up to 128). Runs on the current stream.
     """
     n, k = weight.shape
-    _plain(x, 'x')
-    _check(x.dtype in ACTIVATION_CODES, 'x must be float32, float16, bfloat16, int8 or float8_e4m3fn')
-    device = x.device
-    _check(weight.device == device, 'the weight must be on the device of x')
-    rows = _flat_rows(x, k, 'x')
-    m = rows.shape[0]
-    eight_bit = x.dtype not in FLOAT_CODES
-    for given in (out, residual, bias):
-        if out_dtype is None and given is not None:
-            out_dtype = given.dtype
-    if out_dtype is None:
-        _check(not eight_bit, '8-bit x needs out_dtype, out, residual or bias')
-        out_dtype = x.dtype
-    _check(out_dtype in FLOAT_CODES, 'out_dtype must be float32, float16 or bfloat16')
-    scale_at = 0
-    if x_scale is not None:
-        _plain(x_scale, 'x_scale')
-        _check(x_scale.dtype == torch.float32 and x_scale.numel() == m and x_scale.is_contiguous()
-               and x_scale.device == device, 'x_scale must be contiguous float32 on the device of x, one per row')
-        scale_at = x_scale.data_ptr()
+    x_dtype = x.dtype
+    code = ACTIVATION_CODES.get(x_dtype)
+    _check(code is not None, 'x must be float32, float16, bfloat16, int8 or float8_e4m3fn')
+    index = x.get_device()
+    if not _usable(x, index):
+        _refuse(x, 'x', index)
+    if weight.index != index:
+        _check(False, 'the weight must be on the device of x')
+    x_shape = x.shape
+    if not x_shape or x_shape[-1] != k:
+        _check(False, f'x must have {k} features')
+    x_stride = _row_stride(x, k, 'x')
+    if len(x_shape) == 2:
+        m = x_shape[0]
+        shape = (m, n)
     else:
-        _check(not eight_bit, '8-bit x needs x_scale')
-    shape = x.shape[:-1] + (n,)
-    bias_at = residual_at = residual_stride = 0
+        shape = x_shape[:-1] + (n,)
+        m = x.numel() // k
+    if out_dtype is None:
+        given = out if out is not None else residual if residual is not None else bias
+        _check(given is not None or code <= 2, '8-bit x needs out_dtype, out, residual or bias')
+        out_dtype = x_dtype if given is None else given.dtype
+    out_code = FLOAT_CODES.get(out_dtype)
+    _check(out_code is not None, 'out_dtype must be float32, float16 or bfloat16')
+    scale_at = bias_at = residual_at = residual_stride = 0
+    if x_scale is not None:
+        if not _usable(x_scale, index):
+            _refuse(x_scale, 'x_scale', index)
+        if x_scale.dtype is not torch.float32 or x_scale.numel() != m or not x_scale.is_contiguous():
+            _check(False, 'x_scale must be contiguous float32, one per row')
+        scale_at = x_scale.data_ptr()
+    elif code > 2:
+        _check(False, '8-bit x needs x_scale')
     if bias is not None:
-        _plain(bias, 'bias')
-        _check(bias.shape == (n,) and bias.dtype == out_dtype and bias.is_contiguous() and bias.device == device,
-               'bias must be a contiguous [N] tensor of out_dtype on the device of x')
+        if not _usable(bias, index):
+            _refuse(bias, 'bias', index)
+        if bias.dtype is not out_dtype or bias.shape != (n,) or not bias.is_contiguous():
+            _check(False, 'bias must be a contiguous [N] tensor of out_dtype')
         bias_at = bias.data_ptr()
     if residual is not None:
-        _plain(residual, 'residual')
-        _check(residual.shape == shape and residual.dtype == out_dtype and residual.device == device,
-               'residual must be a [..., N] tensor of out_dtype on the device of x')
-        flat = _flat_rows(residual, n, 'residual')
-        residual_at, residual_stride = flat.data_ptr(), flat.stride(0)
+        if not _usable(residual, index):
+            _refuse(residual, 'residual', index)
+        if residual.dtype is not out_dtype or residual.shape != shape:
+            _check(False, 'residual must be a [..., N] tensor of out_dtype')
+        residual_stride = _row_stride(residual, n, 'residual')
+        residual_at = residual.data_ptr()
     if out is None:
-        out = torch.empty(shape, dtype=out_dtype, device=device)
+        # Shapes given as separate numbers cost torch the least host time.
+        out = torch.empty(*shape, dtype=out_dtype, device=x.device)
         out_at, out_stride = out.data_ptr(), n
     else:
-        _plain(out, 'out')
-        _check(out.shape == shape and out.dtype == out_dtype and out.device == device,
-               'out must be a [..., N] tensor of out_dtype on the device of x')
-        flat = _flat_rows(out, n, 'out')
-        out_at, out_stride = flat.data_ptr(), flat.stride(0)
+        if not _usable(out, index):
+            _refuse(out, 'out', index)
+        _check(out.shape == shape and out.dtype is out_dtype, 'out must be a [..., N] tensor of out_dtype')
+        out_at, out_stride = out.data_ptr(), _row_stride(out, n, 'out')
         _check(m <= 1 or out_stride >= n, 'rows of out must not overlap')
         for other in (x, x_scale, bias, weight.records):
             _check(other is None or not storage_overlaps(out, other), 'out must not alias an input')
         _check(residual is None or (out_at == residual_at and (m <= 1 or out_stride == residual_stride))
                or not storage_overlaps(out, residual), 'out must be the residual itself or not alias it')
-    if m == 0:
-        return out
-    _launch(_native.library().mvq_w4_linear, _native.pack_linear(
-        rows.data_ptr(), rows.stride(0), scale_at, *weight._fixed, bias_at, residual_at, residual_stride,
-        out_at, out_stride, m, ACTIVATION_CODES[x.dtype], FLOAT_CODES[out_dtype]), device.index)
+    if m:
+        _launch(_native.library().mvq_w4_linear, _native.pack_linear(
+            x.data_ptr(), x_stride, scale_at, *weight.fixed, bias_at, residual_at, residual_stride, out_at, out_stride,
+            m, code, out_code), index)
     return out
 
 
@@ -247,17 +271,19 @@ def w4_dequantize(weight: W4Weight, dtype: torch.dtype | None = None, *,
     out: an [N, K] tensor of ``dtype``, rows may be strided. Runs on the current stream.
     """
     n, k = weight.shape
-    _check(weight.device.type == 'cuda', 'the weight must be on a CUDA device')
+    index = weight.index
+    _check(index >= 0, 'the weight must be on a CUDA device')
     dtype = dtype or (out.dtype if out is not None else weight.scale_dtype)
-    _check(dtype in FLOAT_CODES, 'dtype must be float32, float16 or bfloat16')
+    code = FLOAT_CODES.get(dtype)
+    _check(code is not None, 'dtype must be float32, float16 or bfloat16')
     if out is None:
-        out = torch.empty((n, k), dtype=dtype, device=weight.device)
+        out = torch.empty(n, k, dtype=dtype, device=weight.device)
     else:
-        _plain(out, 'out')
-        _check(out.shape == (n, k) and out.dtype == dtype and out.device == weight.device
-               and (k == 1 or out.stride(1) == 1) and (n == 1 or out.stride(0) >= k),
-               'out must be an [N, K] tensor of dtype on the device of the weight, with feature stride 1')
+        if not _usable(out, index):
+            _refuse(out, 'out', index)
+        _check(out.shape == (n, k) and out.dtype == dtype and (k == 1 or out.stride(1) == 1)
+               and (n == 1 or out.stride(0) >= k), 'out must be an [N, K] tensor of dtype with feature stride 1')
         _check(not storage_overlaps(out, weight.records), 'out must not alias the weight')
     _launch(_native.library().mvq_w4_dequantize, _native.pack_dequantize(
-        *weight._fixed, out.data_ptr(), out.stride(0), FLOAT_CODES[dtype]), weight.device.index)
+        *weight.fixed, out.data_ptr(), out.stride(0), code), index)
     return out
