@@ -78,33 +78,45 @@ int check_weight(const void* records, int64_t n, int64_t k, int64_t group, int64
 // Threads and runs of eight per thread for rows of `width` elements.
 struct RowShape {
     int threads;
-    int held;  // runs of eight elements a thread holds: 1, 2, 4 or 8; 0: none, the row is read twice
+    int held;      // runs of eight elements a thread holds: 1, 2, 4 or 8; 0: none, the row is read twice
+    int per_cta;   // rows
 };
 
 // `most`: the most runs that a thread may hold.
 RowShape row_shape(int64_t width, int64_t rows, int sms, int most) {
     const int64_t runs = (width + 7) / 8;
     // Few rows: a thread per run, which spreads the row's latency over the CTA.
-    // Many rows: two runs a thread.
-    int held = rows > 2 * static_cast<int64_t>(sms) ? 2 : 1;
+    // Many rows: two runs a thread and CTAs of at most 512 threads (2048 rows of
+    // 14336: 33.6 us, with at most 256 threads 37.9, with up to 1024 62), or eight
+    // rows a CTA where a warp holds a row (8192 rows of 128: 3.4 us, a CTA each 8.9;
+    // of 896: 9.9 and 10.6).
+    int held = 1;
+    if (rows > 2 * static_cast<int64_t>(sms)) {
+        if (runs <= 128) {
+            while (runs > 32 * held) held *= 2;
+            return {32, held, 8};
+        }
+        for (held = 2; held < most && runs > static_cast<int64_t>(held) * 512;) held *= 2;
+    }
     while (held <= most && runs > static_cast<int64_t>(held) * mvq::max_row_threads(held)) held *= 2;
-    if (held > most) return {mvq::max_row_threads(0), 0};
-    return {static_cast<int>(((runs + held - 1) / held + 31) / 32 * 32), held};
+    if (held > most) return {mvq::max_row_threads(0), 0, 1};
+    return {static_cast<int>(((runs + held - 1) / held + 31) / 32 * 32), held, 1};
 }
 
 template <typename T, int OUT, bool RUNS, template <typename, int, bool, int> class Kernel, typename P>
 cudaError_t launch_row_held(const P& p, RowShape shape, int64_t rows, void* stream) {
-    const dim3 grid(static_cast<unsigned>(rows));
+    const dim3 grid(static_cast<unsigned>((rows + shape.per_cta - 1) / shape.per_cta));
+    const dim3 block(shape.threads, shape.per_cta);
     switch (shape.held) {
-        case 1: return launch(Kernel<T, OUT, RUNS, 1>::get(), grid, shape.threads, 0, 1, stream, p);
-        case 2: return launch(Kernel<T, OUT, RUNS, 2>::get(), grid, shape.threads, 0, 1, stream, p);
+        case 1: return launch(Kernel<T, OUT, RUNS, 1>::get(), grid, block, 0, 1, stream, p);
+        case 2: return launch(Kernel<T, OUT, RUNS, 2>::get(), grid, block, 0, 1, stream, p);
         default: break;
     }
     if constexpr (RUNS) {
-        if (shape.held == 4) return launch(Kernel<T, OUT, RUNS, 4>::get(), grid, shape.threads, 0, 1, stream, p);
-        if (shape.held == 8) return launch(Kernel<T, OUT, RUNS, 8>::get(), grid, shape.threads, 0, 1, stream, p);
+        if (shape.held == 4) return launch(Kernel<T, OUT, RUNS, 4>::get(), grid, block, 0, 1, stream, p);
+        if (shape.held == 8) return launch(Kernel<T, OUT, RUNS, 8>::get(), grid, block, 0, 1, stream, p);
     }
-    return launch(Kernel<T, OUT, RUNS, 0>::get(), grid, shape.threads, 0, 1, stream, p);
+    return launch(Kernel<T, OUT, RUNS, 0>::get(), grid, block, 0, 1, stream, p);
 }
 
 template <typename T, int OUT, template <typename, int, bool, int> class Kernel, typename P>
@@ -263,6 +275,7 @@ int mvq_add_rms_norm(const MvqNormArgs* a, void* stream) try {
     const bool runs = a->hidden % 8 == 0 && wide % 16 == 0 && address(a->out) % out_run == 0 &&
                       (one || a->out_stride_row * (eight ? 1 : size) % out_run == 0);
     mvq::NormParams p = {};
+    p.rows = a->rows;
     p.x = a->x;
     p.x_stride = a->x_stride_row;
     p.residual = a->residual;
@@ -305,6 +318,7 @@ int mvq_silu_mul_quant(const MvqSiluArgs* a, void* stream) try {
     const bool runs = a->width % 8 == 0 && address(a->gate_up) % 16 == 0 && address(a->out) % 8 == 0 &&
                       (one || (a->stride_row * size % 16 == 0 && a->out_stride_row % 8 == 0));
     mvq::SiluParams p = {};
+    p.rows = a->rows;
     p.gate_up = a->gate_up;
     p.stride = a->stride_row;
     p.out = a->out;

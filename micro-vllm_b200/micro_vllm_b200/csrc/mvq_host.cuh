@@ -21,11 +21,11 @@ int cuda_fail(cudaError_t err, const char* what);
 // Programmatic stream serialization (the kernels wait before they read), and a
 // cluster along x where one is asked for.
 template <typename... Params, typename... Args>
-cudaError_t launch(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, int cluster, void* stream,
+cudaError_t launch(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, int cluster, void* stream,
                    Args&&... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
+    cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = static_cast<cudaStream_t>(stream);
     cudaLaunchAttribute attr[2];

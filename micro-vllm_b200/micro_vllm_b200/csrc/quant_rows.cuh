@@ -7,7 +7,7 @@
 // reductions and the store, so each input is read once and each output written
 // once. The norm's maximum needs no second pass over the data: max|y| =
 // rsqrt(...) * max|weight * s|, so the sum of squares and the maximum are
-// reduced together. One CTA per row.
+// reduced together. One CTA per row, or, for many narrow rows, one warp.
 #pragma once
 
 #include <cuda_fp8.h>
@@ -21,6 +21,19 @@ using mv::to_float;
 
 enum : int { kOutSame = 0, kOutI8 = 1, kOutE4M3 = 2 };
 
+// Two fp32 numbers rounded to a pair of T (the first in the low half), and back.
+template <typename T>
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
+    return mv::MmaOp<T>::pack(lo, hi);
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack_pair(uint32_t w) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value)
+        return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    else
+        return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
 // Eight elements of a row. Runs: the eight at 8 c (one or two 16-byte
 // accesses). Elements: the eight at `threads` apart, each checked, for rows
 // that are not aligned or not a multiple of eight wide.
@@ -31,33 +44,72 @@ struct RowAccess {
         return RUNS ? 8 * (j * threads + static_cast<int>(threadIdx.x)) + i
                     : (8 * j + i) * threads + static_cast<int>(threadIdx.x);
     }
-    __device__ __forceinline__ void load(const T* row, int j, float (&v)[8]) const {
+    // Eight elements as they lie in memory, so that several loads can be under way before one is used.
+    struct Raw {
+        uint4 w[sizeof(T) / 2];  // RUNS
+        T e[RUNS ? 1 : 8];       // elements
+    };
+    __device__ __forceinline__ void fetch(const T* row, int j, Raw& r) const {
         if constexpr (RUNS) {
-            if (at(j, 0) < width) {
-                __align__(16) T e[8];
 #pragma unroll
-                for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
-                    reinterpret_cast<uint4*>(e)[i] = reinterpret_cast<const uint4*>(row + at(j, 0))[i];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = to_float<T>(e[i]);
-                return;
+            for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
+                r.w[i] = make_uint4(0, 0, 0, 0);
+                if (at(j, 0) < width) r.w[i] = reinterpret_cast<const uint4*>(row + at(j, 0))[i];
             }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = 0.0f;
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = at(j, i) < width ? to_float<T>(row[at(j, i)]) : 0.0f;
+            for (int i = 0; i < 8; ++i) r.e[i] = at(j, i) < width ? row[at(j, i)] : from_float<T>(0.0f);
+        }
+    }
+    __device__ __forceinline__ void expand(const Raw& r, float (&v)[8]) const {
+        if constexpr (!RUNS) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = to_float<T>(r.e[i]);
+        } else if constexpr (sizeof(T) == 4) {
+            v[0] = __uint_as_float(r.w[0].x), v[1] = __uint_as_float(r.w[0].y), v[2] = __uint_as_float(r.w[0].z);
+            v[3] = __uint_as_float(r.w[0].w), v[4] = __uint_as_float(r.w[1].x), v[5] = __uint_as_float(r.w[1].y);
+            v[6] = __uint_as_float(r.w[1].z), v[7] = __uint_as_float(r.w[1].w);
+        } else {
+            const uint32_t words[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = unpack_pair<T>(words[i]);
+                v[2 * i] = f.x, v[2 * i + 1] = f.y;
+            }
+        }
+    }
+    __device__ __forceinline__ void load(const T* row, int j, float (&v)[8]) const {
+        Raw r;
+        fetch(row, j, r);
+        expand(r, v);
+    }
+    // Stores v rounded to T (if `row` is not null) and leaves the rounded values in v.
+    __device__ __forceinline__ void round_store(T* row, int j, float (&v)[8]) const {
+        if constexpr (RUNS && sizeof(T) == 2) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w[i] = pack_pair<T>(v[2 * i], v[2 * i + 1]);
+                const float2 f = unpack_pair<T>(w[i]);
+                v[2 * i] = f.x, v[2 * i + 1] = f.y;
+            }
+            if (row && at(j, 0) < width)
+                *reinterpret_cast<uint4*>(row + at(j, 0)) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = to_float<T>(from_float<T>(v[i]));
+            if (row) store(row, j, v);
         }
     }
     __device__ __forceinline__ void store(T* row, int j, const float (&v)[8]) const {
         if constexpr (RUNS) {
-            if (at(j, 0) < width) {
-                __align__(16) T e[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) e[i] = from_float<T>(v[i]);
-#pragma unroll
-                for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
-                    reinterpret_cast<uint4*>(row + at(j, 0))[i] = reinterpret_cast<const uint4*>(e)[i];
+            if (at(j, 0) >= width) return;
+            if constexpr (sizeof(T) == 4) {
+                reinterpret_cast<float4*>(row + at(j, 0))[0] = make_float4(v[0], v[1], v[2], v[3]);
+                reinterpret_cast<float4*>(row + at(j, 0))[1] = make_float4(v[4], v[5], v[6], v[7]);
+            } else {
+                *reinterpret_cast<uint4*>(row + at(j, 0)) = make_uint4(pack_pair<T>(v[0], v[1]), pack_pair<T>(v[2], v[3]),
+                                                                       pack_pair<T>(v[4], v[5]), pack_pair<T>(v[6], v[7]));
             }
         } else {
 #pragma unroll
@@ -65,30 +117,31 @@ struct RowAccess {
                 if (at(j, i) < width) row[at(j, i)] = from_float<T>(v[i]);
         }
     }
-    // Eight 8-bit values (already scaled).
+    // Eight finite values, scaled already, as 8-bit numbers.
     template <int OUT>
     __device__ __forceinline__ void store8(uint8_t* row, int j, const float (&v)[8]) const {
-        uint32_t b[8];
-        if constexpr (OUT == kOutI8) {
+        uint32_t w[2];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) b[i] = static_cast<uint32_t>(__float2int_rn(v[i])) & 0xffu;
-        } else {
+        for (int i = 0; i < 2; ++i) {
+            if constexpr (OUT == kOutI8) {
+                // 1.5 2^23 + v rounds v to an integer, whose low byte is the number's lowest.
+                uint32_t b[4];
 #pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-                const uint32_t two = __nv_cvt_float2_to_fp8x2(make_float2(v[i], v[i + 1]), __NV_SATFINITE, __NV_E4M3);
-                b[i] = two & 0xffu;
-                b[i + 1] = two >> 8;
+                for (int e = 0; e < 4; ++e) b[e] = __float_as_uint(v[4 * i + e] + 12582912.0f);
+                w[i] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+            } else {
+                uint16_t lo, hi;
+                asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(v[4 * i + 1]), "f"(v[4 * i]));
+                asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(v[4 * i + 3]), "f"(v[4 * i + 2]));
+                w[i] = static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
             }
         }
         if constexpr (RUNS) {
-            if (at(j, 0) < width)
-                *reinterpret_cast<uint2*>(row + at(j, 0)) =
-                    make_uint2(b[0] | (b[1] << 8) | (b[2] << 16) | (b[3] << 24),
-                               b[4] | (b[5] << 8) | (b[6] << 16) | (b[7] << 24));
+            if (at(j, 0) < width) *reinterpret_cast<uint2*>(row + at(j, 0)) = make_uint2(w[0], w[1]);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (at(j, i) < width) row[at(j, i)] = static_cast<uint8_t>(b[i]);
+                if (at(j, i) < width) row[at(j, i)] = static_cast<uint8_t>(w[i >> 2] >> (8 * (i & 3)));
         }
     }
 };
@@ -120,25 +173,34 @@ __device__ __forceinline__ float2 block_sum_max(float sum, float top) {
     return all;
 }
 
-// Scale of a row whose largest |y| is `amax`, and what takes a value v with
-// y = v * amax / top_v to its 8-bit number: v * mul.x * mul.y. mul.x is a power
-// of two that keeps top / top_v finite for tiny rows.
+// What turns a row's values v (y = v * amax / top_v) into its 8-bit numbers: v
+// times `mul`, or, where top / top_v would overflow, v * 2^100 times `mul`. A
+// mul of zero: the row has no scale (zeros, or a NaN or an infinity among them).
+struct RowScale {
+    float scale, mul;
+    bool tiny;
+};
 template <int OUT>
-__device__ __forceinline__ float row_scale(float amax, float top_v, float2* mul) {
+__device__ __forceinline__ RowScale row_scale(float amax, float top_v) {
     constexpr float kTop = OUT == kOutI8 ? 127.0f : 448.0f;
-    const float scale = amax < INFINITY ? amax / kTop : __int_as_float(0x7fffffff);
-    const float up = top_v < 0x1p-100f ? 0x1p+100f : 1.0f;
-    *mul = scale > 0.0f ? make_float2(up, kTop / (top_v * up)) : make_float2(0.0f, 0.0f);
-    return scale;
+    RowScale s;
+    s.scale = amax < INFINITY ? amax / kTop : __int_as_float(0x7fffffff);
+    s.tiny = top_v < 0x1p-100f;
+    s.mul = s.scale > 0.0f ? kTop / (s.tiny ? top_v * 0x1p+100f : top_v) : 0.0f;
+    return s;
 }
-
-template <int OUT>
-__device__ __forceinline__ float scaled(float v, float2 mul) {
-    // A row without a scale gives zeros, whatever its values (NaN and infinities among them).
-    return mul.y == 0.0f ? 0.0f : v * mul.x * mul.y;
+__device__ __forceinline__ void apply_scale(const RowScale& s, float (&v)[8]) {
+    if (s.mul == 0.0f || s.tiny) {  // the same for the whole row
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = s.mul == 0.0f ? 0.0f : v[i] * 0x1p+100f * s.mul;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= s.mul;
+    }
 }
 
 struct NormParams {
+    int64_t rows;
     const void* x;
     int64_t x_stride;
     const void* residual;
@@ -161,33 +223,35 @@ __global__ void __launch_bounds__(max_row_threads(C)) add_rms_norm_kernel(const 
     mv::wait_for_prior_grid();
     mv::allow_next_grid();
     const RowAccess<T, RUNS> at{p.hidden, static_cast<int>(blockDim.x)};
-    const int64_t row = blockIdx.x;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+    if (row >= p.rows) return;  // with several rows per CTA, each has one warp and waits for no other
     const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
     const T* residual = p.residual ? static_cast<const T*>(p.residual) + row * p.residual_stride : nullptr;
     T* residual_out = p.residual_out ? static_cast<T*>(p.residual_out) + row * p.residual_out_stride : nullptr;
     const T* weight = static_cast<const T*>(p.weight);
     T* out = static_cast<T*>(p.out) + row * p.out_stride;
     uint8_t* out8 = static_cast<uint8_t*>(p.out) + row * p.out_stride;
-    const auto add = [&](int j, float (&v)[8]) {  // s of run j, x's values being in v
+    using Raw = typename RowAccess<T, RUNS>::Raw;
+    const auto add = [&](int j, float (&v)[8], const Raw& r, T* to) {  // s of run j, x's values being in v
         if (!residual) return;
         float e[8];
-        at.load(residual, j, e);
+        at.expand(r, e);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = to_float<T>(from_float<T>(__fadd_rn(v[i], e[i])));
+        for (int i = 0; i < 8; ++i) v[i] = __fadd_rn(v[i], e[i]);
+        at.round_store(to, j, v);
     };
-    const auto weigh = [&](int j, float (&v)[8]) {
+    const auto weigh = [&](const Raw& r, float (&v)[8]) {
         float w[8];
-        at.load(weight, j, w);
+        at.expand(r, w);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] *= w[i];
     };
     float sum = 0.0f, top = 0.0f;
-    const auto gather = [&](int j, float (&v)[8]) {  // v: x in, weight * s out
-        add(j, v);
-        if (residual_out) at.store(residual_out, j, v);
+    const auto gather = [&](int j, float (&v)[8], const Raw& r, const Raw& w) {  // v: x in, weight * s out
+        add(j, v, r, residual_out);
 #pragma unroll
         for (int i = 0; i < 8; ++i) sum = fmaf(v[i], v[i], sum);
-        weigh(j, v);
+        weigh(w, v);
         if (OUT != kOutSame) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(v[i]));
@@ -196,22 +260,34 @@ __global__ void __launch_bounds__(max_row_threads(C)) add_rms_norm_kernel(const 
     const int turns = (p.hidden + 8 * static_cast<int>(blockDim.x) - 1) / (8 * static_cast<int>(blockDim.x));
     float v[C ? C : 1][8];
     if constexpr (C > 0) {
+        Raw rx[C], rr[C], rw[C];
 #pragma unroll
-        for (int j = 0; j < C; ++j) at.load(x, j, v[j]);
+        for (int j = 0; j < C; ++j) {
+            at.fetch(x, j, rx[j]);
+            if (residual) at.fetch(residual, j, rr[j]);
+        }
 #pragma unroll
-        for (int j = 0; j < C; ++j) gather(j, v[j]);
+        for (int j = 0; j < C; ++j) at.fetch(weight, j, rw[j]);
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            at.expand(rx[j], v[j]);
+            gather(j, v[j], rr[j], rw[j]);
+        }
     } else {
         for (int j = 0; j < turns; ++j) {
+            Raw r, w;
             at.load(x, j, v[0]);
-            gather(j, v[0]);
+            if (residual) at.fetch(residual, j, r);
+            at.fetch(weight, j, w);
+            gather(j, v[0], r, w);
         }
     }
     const float2 all = block_sum_max(sum, top);
     const float r = rsqrtf(all.x / static_cast<float>(p.hidden) + p.eps);
-    float2 mul = make_float2(r, 1.0f);
+    RowScale scale;
     if constexpr (OUT != kOutSame) {
-        const float scale = row_scale<OUT>(all.y * r, all.y, &mul);
-        if (threadIdx.x == 0) p.scales[row] = scale;
+        scale = row_scale<OUT>(all.y * r, all.y);
+        if (threadIdx.x == 0) p.scales[row] = scale.scale;
     }
     const auto finish = [&](int j, float (&v)[8]) {
         if constexpr (OUT == kOutSame) {
@@ -219,8 +295,7 @@ __global__ void __launch_bounds__(max_row_threads(C)) add_rms_norm_kernel(const 
             for (int i = 0; i < 8; ++i) v[i] *= r;
             at.store(out, j, v);
         } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = scaled<OUT>(v[i], mul);
+            apply_scale(scale, v);
             at.template store8<OUT>(out8, j, v);
         }
     };
@@ -231,14 +306,20 @@ __global__ void __launch_bounds__(max_row_threads(C)) add_rms_norm_kernel(const 
         for (int j = 0; j < turns; ++j) {
             // The sum that this thread stored, where there is one: it may lie over x or the residual.
             at.load(residual_out ? residual_out : x, j, v[0]);
-            if (!residual_out) add(j, v[0]);
-            weigh(j, v[0]);
+            Raw r;
+            if (residual && !residual_out) {
+                at.fetch(residual, j, r);
+                add(j, v[0], r, nullptr);
+            }
+            at.fetch(weight, j, r);
+            weigh(r, v[0]);
             finish(j, v[0]);
         }
     }
 }
 
 struct SiluParams {
+    int64_t rows;
     const void* gate_up;
     int64_t stride;
     void* out;
@@ -252,16 +333,27 @@ __global__ void __launch_bounds__(max_row_threads(C)) silu_mul_quant_kernel(cons
     mv::wait_for_prior_grid();
     mv::allow_next_grid();
     const RowAccess<T, RUNS> at{p.width, static_cast<int>(blockDim.x)};
-    const int64_t row = blockIdx.x;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+    if (row >= p.rows) return;  // with several rows per CTA, each has one warp and waits for no other
     const T* gate = static_cast<const T*>(p.gate_up) + row * p.stride;
     uint8_t* out = static_cast<uint8_t*>(p.out) + row * p.out_stride;
     float top = 0.0f;
+    const auto gated = [&](float (&v)[8], const float (&u)[8]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            // 2^(-g log2 e) and 1 / (1 + it), each within two units of fp32's last place; an
+            // exponential past its range makes the value a zero, as the division would.
+            float e, d;
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v[i] * -1.4426950408889634f));
+            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(1.0f + e));
+            v[i] = v[i] * d * u[i];
+        }
+    };
     const auto value = [&](int j, float (&v)[8]) {
         float u[8];
         at.load(gate, j, v);
         at.load(gate + p.width, j, u);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = __fdividef(v[i], 1.0f + __expf(-v[i])) * u[i];
+        gated(v, u);
     };
     const auto measure = [&](const float (&v)[8]) {
 #pragma unroll
@@ -270,9 +362,18 @@ __global__ void __launch_bounds__(max_row_threads(C)) silu_mul_quant_kernel(cons
     const int turns = (p.width + 8 * static_cast<int>(blockDim.x) - 1) / (8 * static_cast<int>(blockDim.x));
     float v[C ? C : 1][8];
     if constexpr (C > 0) {
+        typename RowAccess<T, RUNS>::Raw rg[C], ru[C];
 #pragma unroll
         for (int j = 0; j < C; ++j) {
-            value(j, v[j]);
+            at.fetch(gate, j, rg[j]);
+            at.fetch(gate + p.width, j, ru[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            float u[8];
+            at.expand(rg[j], v[j]);
+            at.expand(ru[j], u);
+            gated(v[j], u);
             measure(v[j]);
         }
     } else {
@@ -282,12 +383,10 @@ __global__ void __launch_bounds__(max_row_threads(C)) silu_mul_quant_kernel(cons
         }
     }
     const float2 all = block_sum_max(0.0f, top);
-    float2 mul;
-    const float scale = row_scale<OUT>(all.y, all.y, &mul);
-    if (threadIdx.x == 0) p.scales[row] = scale;
+    const RowScale scale = row_scale<OUT>(all.y, all.y);
+    if (threadIdx.x == 0) p.scales[row] = scale.scale;
     const auto finish = [&](int j, float (&v)[8]) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = scaled<OUT>(v[i], mul);
+        apply_scale(scale, v);
         at.template store8<OUT>(out, j, v);
     };
     if constexpr (C > 0) {

@@ -602,19 +602,52 @@ __global__ void __launch_bounds__(kThreads, NB == 4 ? 2 : 4) w4_linear_kernel(co
 }
 
 // W written out, rounded once: a warp per record. Bound by the output's bytes.
+// A code's distance from its zero point is exact in 16 bits, and its product
+// with a scale has at most 4 + 11 bits, so that a 16-bit product with a scale of
+// the output's type (`same`) rounds exactly as the fp32 product does.
 template <typename T>
-__global__ void __launch_bounds__(256)
+struct PairOf;
+template <>
+struct PairOf<__half> {
+    using Kind = Act<kF16>;
+    using Pair = __half2;
+};
+template <>
+struct PairOf<__nv_bfloat16> {
+    using Kind = Act<kBF16>;
+    using Pair = __nv_bfloat162;
+};
+template <>
+struct PairOf<float> : PairOf<__nv_bfloat16> {};
+
+constexpr int kDequantizeWarps = 8;
+
+template <typename T>
+__global__ void __launch_bounds__(kDequantizeWarps * 32)
 w4_dequantize_kernel(const uint8_t* records, int64_t total, int chunks, int record_bytes, int group, int has_zeros,
                      int scale_bf16, int n, int k, T* out, int64_t out_stride, int runs) {
+    using Kind = typename PairOf<T>::Kind;
+    using Pair = typename PairOf<T>::Pair;
+    constexpr bool kBf16 = std::is_same<Kind, Act<kBF16>>::value;
     mv::wait_for_prior_grid();
     mv::allow_next_grid();
-    const int64_t id = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    const int64_t id = static_cast<int64_t>(blockIdx.x) * kDequantizeWarps + (threadIdx.x >> 5);
     if (id >= total) return;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int64_t tile = id / chunks;
     const int k0 = static_cast<int>(id - tile * chunks) * kChunk;
     const uint8_t* rec = records + id * record_bytes;
     const int group_runs = group / 32, groups = kChunk / group;
+    const bool same = sizeof(T) == 2 && (scale_bf16 != 0) == kBf16;
+    // Rows that are not aligned go out through shared memory, so that a warp
+    // stores 32 columns of one row at a time.
+    __shared__ T rows_out[sizeof(T) == 2 ? kDequantizeWarps : 1][sizeof(T) == 2 ? 64 * 34 : 1];
+    uint4 codes[4][2];
+#pragma unroll
+    for (int h = 0; h < 4; ++h)
+#pragma unroll
+        for (int rp = 0; rp < 2; ++rp) codes[h][rp] = __ldg(reinterpret_cast<const uint4*>(rec) + (h * 2 + rp) * 32 + lane);
+#pragma unroll
     for (int h = 0; h < 4; ++h) {
         const int gi = h / group_runs;
         // Two lanes trade words, so that each holds eight columns in a row: the
@@ -622,7 +655,7 @@ w4_dequantize_kernel(const uint8_t* records, int64_t total, int chunks, int reco
         const int c0 = k0 + 32 * h + 16 * (t & 1) + 4 * (t & 2);
 #pragma unroll
         for (int rp = 0; rp < 2; ++rp) {
-            uint4 w = __ldg(reinterpret_cast<const uint4*>(rec) + (h * 2 + rp) * 32 + lane);
+            uint4 w = codes[h][rp];
             const uint32_t got0 = __shfl_xor_sync(0xffffffffu, t & 1 ? w.x : w.y, 1);
             const uint32_t got1 = __shfl_xor_sync(0xffffffffu, t & 1 ? w.z : w.w, 1);
             if (t & 1) w.x = got0, w.z = got1;
@@ -632,33 +665,81 @@ w4_dequantize_kernel(const uint8_t* records, int64_t total, int chunks, int reco
             if (has_zeros) z = __ldg(reinterpret_cast<const uint32_t*>(rec + kCodeBytes + groups * 128 + gi * 64 + g * 8 + rp * 4));
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-                const float2 sc = scale_pair(q ? s.y : s.x, scale_bf16);
-                const uint32_t w0 = q ? w.z : w.x, w1 = q ? w.w : w.y;
+                const uint32_t scales = q ? s.y : s.x;
+                const uint32_t zl = Kind::zero_low(8 + static_cast<int8_t>(z >> (16 * q)));
+                const uint32_t zh = Kind::zero_high(8 + static_cast<int8_t>(z >> (16 * q + 8)));
+                uint32_t a[2][4];  // per quad: columns 0 1 of row g, of row g + 8, columns 2 3 of row g, of row g + 8
+                Kind::weights(q ? w.z : w.x, zl, zh, a[0]);
+                Kind::weights(q ? w.w : w.y, zl, zh, a[1]);
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     const int64_t row = tile * kTileRows + 32 * rp + 16 * q + 8 * half + g;
-                    if (row >= n) continue;
-                    const float scale = half ? sc.y : sc.x;
-                    const int zero = static_cast<int8_t>(z >> (16 * q + 8 * half));
-                    __align__(16) T v[8];
+                    if (runs && row >= n) continue;
+                    float f[8];
+                    uint32_t v[4];
+                    if (same) {
+                        // Kind's power of two goes to the scale first, which is exact.
+                        const uint32_t up = kBf16 ? 0x45004500u : 0x3c003c00u;  // 2^11, 1
+                        const uint32_t bits = __byte_perm(scales, 0, half ? 0x3232 : 0x1010);
+                        const Pair sc = __hmul2(*reinterpret_cast<const Pair*>(&bits), *reinterpret_cast<const Pair*>(&up));
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const uint32_t word = i < 4 ? w0 : w1;
-                        const int s_at = i & 3, byte = s_at == 1 ? 2 : s_at == 2 ? 1 : s_at;
-                        const int code = static_cast<int>(((word >> (8 * byte + 4 * half)) & 15u) ^ 8u) - 8;
-                        v[i] = from_float<T>(static_cast<float>(code - zero) * scale);
+                        for (int i = 0; i < 4; ++i) {
+                            Pair d = *reinterpret_cast<const Pair*>(&a[i >> 1][half + 2 * (i & 1)]);
+                            d = __hmul2(d, sc);
+                            v[i] = *reinterpret_cast<const uint32_t*>(&d);
+                        }
+                    } else {
+                        const float2 both = scale_pair(scales, scale_bf16);
+                        const float scale = half ? both.y : both.x;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint32_t pair = a[i >> 1][half + 2 * (i & 1)];
+                            const float2 d = scale_pair(pair, kBf16);
+                            f[2 * i] = d.x * Kind::kScale * scale, f[2 * i + 1] = d.y * Kind::kScale * scale;
+                        }
+                        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) v[i] = mv::MmaOp<T>::pack(f[2 * i], f[2 * i + 1]);
+                        }
                     }
                     T* dst = out + row * out_stride + c0;
                     if (runs && c0 + 8 <= k) {
+                        if constexpr (sizeof(T) == 2) {
+                            *reinterpret_cast<uint4*>(dst) = make_uint4(v[0], v[1], v[2], v[3]);
+                        } else {
+                            reinterpret_cast<float4*>(dst)[0] = make_float4(f[0], f[1], f[2], f[3]);
+                            reinterpret_cast<float4*>(dst)[1] = make_float4(f[4], f[5], f[6], f[7]);
+                        }
+                    } else if (runs || sizeof(T) == 4) {
 #pragma unroll
-                        for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
-                            reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(v)[i];
-                    } else {
+                        for (int i = 0; i < 8; ++i) {
+                            if (row < n && c0 + i < k) {
+                                if constexpr (sizeof(T) == 2) {
+                                    const uint16_t bits = static_cast<uint16_t>(v[i >> 1] >> (16 * (i & 1)));
+                                    dst[i] = *reinterpret_cast<const T*>(&bits);
+                                } else {
+                                    dst[i] = f[i];
+                                }
+                            }
+                        }
+                    } else if constexpr (sizeof(T) == 2) {
+                        uint32_t* at = reinterpret_cast<uint32_t*>(
+                            &rows_out[threadIdx.x >> 5][(32 * rp + 16 * q + 8 * half + g) * 34 + 16 * (t & 1) + 4 * (t & 2)]);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            if (c0 + i < k) dst[i] = v[i];
+                        for (int i = 0; i < 4; ++i) at[i] = v[i];
                     }
                 }
+            }
+        }
+        if constexpr (sizeof(T) == 2) {
+            if (!runs) {
+                __syncwarp();
+                const int column = k0 + 32 * h + lane;
+                T* dst = out + tile * kTileRows * out_stride + column;
+                const int rows_here = min(kTileRows, static_cast<int>(n - tile * kTileRows));
+                if (column < k)
+                    for (int row = 0; row < rows_here; ++row) dst[row * out_stride] = rows_out[threadIdx.x >> 5][row * 34 + lane];
+                __syncwarp();
             }
         }
     }
