@@ -10,49 +10,60 @@ namespace {
 
 // How a call is cut up (see w4_linear_kernel).
 struct LinearPlan {
-    int nb;       // tokens / 8 per pass over the records
-    int ksplit;
-    int cluster;
-    int stages;
+    int ksplit, cluster, stages;
     int64_t x_chunks;
-    size_t ring_bytes;
-    size_t smem;
+    size_t ring_bytes, smem;
 };
 
+// The cut with the least estimated time. A CTA costs `start` (its launch, x's
+// part of its run, the joining of its sums) and its warps' chunks; an SM takes
+// its share of the CTAs, and fewer than twelve warps on it do not hide a
+// warp's own latency. The constants (us) are fitted to measured calls of 896 x
+// 1152 to 8192 x 57344 at 1 to 8 tokens: at one token four warps per tile are
+// best (3584 x 28672: 16.2 us, one warp per tile 17.7), at eight one warp per
+// tile and clusters, which share the staged x (21.7 and 28 us).
 LinearPlan linear_plan(int64_t m, int64_t chunks, int64_t tiles, int kind, int record, int sms) {
-    LinearPlan plan;
-    plan.nb = m <= 8 || kind == kF32 ? 1 : m <= 16 ? 2 : 4;
-    const int64_t tokens = std::min<int64_t>(m, 8 * plan.nb);
-    const int64_t blocks = (m + 8 * plan.nb - 1) / (8 * plan.nb);
+    const int64_t tokens = std::min<int64_t>(m, kTokens);
+    const int64_t blocks = (m + kTokens - 1) / kTokens;
     const int64_t x_chunk = tokens * (kind == kF32 ? 768 : kind == kI8 ? 128 : 256);
-    plan.ksplit = kWarps;
-    plan.cluster = 1;
-    plan.stages = 3;
+    const double chunk = kind == kI8 ? 0.06 + 0.004 * tokens : kind == kF32 ? 0.25 : 0.11 + 0.007 * tokens;
+    LinearPlan best = {};
+    double least = 0.0;
+    for (int ksplit = 1; ksplit <= kWarps; ksplit *= 2) {
+        const int64_t groups = (tiles + kWarps / ksplit - 1) / (kWarps / ksplit);
+        for (int cluster = 1; cluster <= 8 && cluster <= chunks; cluster *= 2) {
+            const int64_t run = (chunks + cluster - 1) / cluster;
+            const int64_t per_warp = (run + ksplit - 1) / ksplit;
+            const double per_sm = static_cast<double>((groups * cluster * blocks + sms - 1) / sms);
+            const double start = 0.7 + 0.006 * tokens * run + 0.02 * tokens;
+            const double busy = kWarps * std::min(per_sm, 4.0);
+            const double time = per_sm * (start + kWarps * per_warp * chunk * std::max(1.0, 12.0 / busy)) +
+                                (cluster > 1 ? 0.6 : 0.0);
+            if (best.cluster == 0 || time < least) {
+                least = time;
+                best.ksplit = ksplit;
+                best.cluster = cluster;
+                best.stages = per_sm >= 4.0 ? 2 : 3;  // four CTAs per SM, or deeper rings
+            }
+        }
+    }
 #ifdef MVQ_TUNE
-    if (getenv("KS")) plan.ksplit = atoi(getenv("KS"));
-    if (getenv("CL")) plan.cluster = atoi(getenv("CL"));
-    if (getenv("ST")) plan.stages = atoi(getenv("ST"));
-    if (!getenv("CL"))
+    if (getenv("KS")) best.ksplit = atoi(getenv("KS"));
+    if (getenv("CL")) best.cluster = atoi(getenv("CL"));
+    if (getenv("ST")) best.stages = atoi(getenv("ST"));
 #endif
-    while (plan.cluster < 8 && tiles * blocks * plan.cluster < 3 * static_cast<int64_t>(sms) &&
-           chunks > kWarps * plan.cluster)
-        plan.cluster *= 2;
-    const int64_t run = (chunks + plan.cluster - 1) / plan.cluster;
-    int64_t most = 32 * 1024;
-#ifdef MVQ_TUNE
-    if (getenv("XB")) most = atoi(getenv("XB"));
-#endif
-    plan.x_chunks = std::max<int64_t>(1, most / x_chunk / plan.ksplit) * plan.ksplit;
-    plan.x_chunks = std::min<int64_t>(plan.x_chunks, (run + plan.ksplit - 1) / plan.ksplit * plan.ksplit);
-    plan.ring_bytes = std::max<size_t>(plan.stages * record, plan.nb * 8 * kPartStride * 4);
-    plan.ring_bytes = (plan.ring_bytes + 127) / 128 * 128;
-    plan.smem = kWarps * plan.ring_bytes + plan.x_chunks * x_chunk;
-    return plan;
+    const int64_t run = (chunks + best.cluster - 1) / best.cluster;
+    best.x_chunks = std::max<int64_t>(1, 16 * 1024 / x_chunk / best.ksplit) * best.ksplit;
+    best.x_chunks = std::min<int64_t>(best.x_chunks, (run + best.ksplit - 1) / best.ksplit * best.ksplit);
+    best.ring_bytes = std::max<size_t>(best.stages * record, kTokens * kPartStride * 4);
+    best.ring_bytes = (best.ring_bytes + 127) / 128 * 128;
+    best.smem = kWarps * best.ring_bytes + best.x_chunks * x_chunk;
+    return best;
 }
 
-template <int KIND, int NB, int GROUP, bool ZEROS>
+template <int KIND, int GROUP, bool ZEROS>
 int launch_linear(LinearParams p, const LinearPlan& plan, int device, void* stream) {
-    auto kernel = w4_linear_kernel<KIND, NB, GROUP, ZEROS>;
+    auto kernel = w4_linear_kernel<KIND, GROUP, ZEROS>;
     static std::mutex mutex;
     static bool ready[kMaxDevices];
     {
@@ -67,7 +78,7 @@ int launch_linear(LinearParams p, const LinearPlan& plan, int device, void* stre
             ready[device] = true;
         }
     }
-    const int64_t blocks = (static_cast<int64_t>(p.m) + 8 * NB - 1) / (8 * NB);
+    const int64_t blocks = (static_cast<int64_t>(p.m) + kTokens - 1) / kTokens;
     if (blocks > 65535) return fail(MVQ_ERR_UNSUPPORTED, "too many rows of x for one call");
     const int per_cta = kWarps / plan.ksplit;
     const int64_t ctas = (static_cast<int64_t>(p.tiles) + per_cta - 1) / per_cta * plan.cluster;
@@ -82,27 +93,23 @@ int launch_linear(LinearParams p, const LinearPlan& plan, int device, void* stre
     return err == cudaSuccess ? MVQ_OK : cuda_fail(err, "4-bit linear kernel launch");
 }
 
-template <int KIND, int NB>
+template <int KIND>
 int launch_linear_group(const LinearParams& p, const LinearPlan& plan, int group, bool zeros, int device,
                         void* stream) {
     switch (group * 2 + zeros) {
-        case 64: return launch_linear<KIND, NB, 32, false>(p, plan, device, stream);
-        case 65: return launch_linear<KIND, NB, 32, true>(p, plan, device, stream);
-        case 128: return launch_linear<KIND, NB, 64, false>(p, plan, device, stream);
-        case 129: return launch_linear<KIND, NB, 64, true>(p, plan, device, stream);
-        case 256: return launch_linear<KIND, NB, 128, false>(p, plan, device, stream);
-        default: return launch_linear<KIND, NB, 128, true>(p, plan, device, stream);
+        case 64: return launch_linear<KIND, 32, false>(p, plan, device, stream);
+        case 65: return launch_linear<KIND, 32, true>(p, plan, device, stream);
+        case 128: return launch_linear<KIND, 64, false>(p, plan, device, stream);
+        case 129: return launch_linear<KIND, 64, true>(p, plan, device, stream);
+        case 256: return launch_linear<KIND, 128, false>(p, plan, device, stream);
+        default: return launch_linear<KIND, 128, true>(p, plan, device, stream);
     }
 }
 
 template <int KIND>
 int launch_linear_kind(const LinearParams& p, int group, bool zeros, int device, int sms, void* stream) {
     const LinearPlan plan = linear_plan(p.m, p.chunks, p.tiles, KIND, record_size(group, zeros), sms);
-    if constexpr (KIND != kF32) {
-        if (plan.nb == 4) return launch_linear_group<KIND, 4>(p, plan, group, zeros, device, stream);
-        if (plan.nb == 2) return launch_linear_group<KIND, 2>(p, plan, group, zeros, device, stream);
-    }
-    return launch_linear_group<KIND, 1>(p, plan, group, zeros, device, stream);
+    return launch_linear_group<KIND>(p, plan, group, zeros, device, stream);
 }
 
 }  // namespace

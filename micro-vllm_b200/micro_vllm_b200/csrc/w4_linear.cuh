@@ -19,6 +19,8 @@
 
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "mv_device.cuh"
 
 namespace mvq {
@@ -31,6 +33,7 @@ constexpr int kChunk = 128;
 constexpr int kCodeBytes = kTileRows * kChunk / 2;
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
+constexpr int kTokens = 8;  // per pass over the records: the columns of one mma.sync tile
 // Row stride of the partial sums [token][64 weight rows] in shared memory, in
 // floats: 68 keeps the eight rows and four token pairs that a warp stores at
 // once in different banks.
@@ -313,14 +316,14 @@ __device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
 }
 
 // A CTA's four warps take 4 / ksplit tiles of 64 weight rows and, with the other
-// CTAs of their cluster, a block of 8 NB tokens. The columns' chunks go to the
+// CTAs of their cluster, up to eight tokens. The columns' chunks go to the
 // cluster's CTAs as runs, within a CTA to the tile's ksplit warps in turn. x's
 // part of the run is staged in shared memory once, as operand numbers; each warp
 // streams its records through a ring of its own (cp.async and no barrier: a warp
 // reads what its own lanes copied) and sums all 64 rows for all tokens; the
 // partial sums meet in (distributed) shared memory and are added in a fixed order.
-template <int KIND, int NB, int GROUP, bool ZEROS>
-__global__ void __launch_bounds__(kThreads, NB == 4 ? 2 : 4) w4_linear_kernel(const LinearParams p) {
+template <int KIND, int GROUP, bool ZEROS>
+__global__ void __launch_bounds__(kThreads, 4) w4_linear_kernel(const LinearParams p) {
     using A = Act<KIND>;
     constexpr int kGroupRuns = GROUP / 32;    // 32-column runs per group
     constexpr int kGroups = kChunk / GROUP;   // groups per chunk
@@ -333,8 +336,8 @@ __global__ void __launch_bounds__(kThreads, NB == 4 ? 2 : 4) w4_linear_kernel(co
     const int rank = p.cluster > 1 ? static_cast<int>(cluster_rank()) : 0;
     const int64_t tile0 = static_cast<int64_t>(blockIdx.x) / p.cluster * (kWarps / p.ksplit);
     const int64_t tile = tile0 + warp / p.ksplit;
-    const int token0 = blockIdx.y * (8 * NB);
-    const int tokens = min(8 * NB, p.m - token0);
+    const int token0 = blockIdx.y * kTokens;
+    const int tokens = min(kTokens, p.m - token0);
     // This CTA's run of chunks, and this warp's among them: begin + kpart, + ksplit, ...
     const int begin = static_cast<int>(static_cast<int64_t>(p.chunks) * rank / p.cluster);
     const int end = static_cast<int>(static_cast<int64_t>(p.chunks) * (rank + 1) / p.cluster);
@@ -370,44 +373,55 @@ __global__ void __launch_bounds__(kThreads, NB == 4 ? 2 : 4) w4_linear_kernel(co
     // x: [chunk][h][plane][t][token] two quads, the columns 16 e + 4 t of h, for x_chunks chunks from `from`.
     const int plane_bytes = 4 * tokens * kRunBytes;
     const int x_size = p.x_dtype == kF32 ? 4 : p.x_dtype >= kI8 ? 1 : 2;
-    const auto stage_x = [&](int from) {
-        const int runs = min(p.x_chunks, end - begin - from) * 16;  // runs of eight of a token: chunk, h, t
-        for (int token = 0; token < tokens; ++token) {
-            const uint8_t* row = static_cast<const uint8_t*>(p.x) + (token0 + token) * p.x_stride * x_size;
+    const auto stage = [&](auto count, int from, int runs) {
+        constexpr int kTogether = decltype(count)::value;
+        for (int first_token = 0; first_token < tokens; first_token += kTogether) {
             for (int run = threadIdx.x; run < runs; run += kThreads) {
-                uint32_t r[kPlanes][kRunBytes / 4];
-                load_run<KIND>(p, row, (begin + from) * kChunk + run * 8, p.k, r);
-                // The run's two quads go to lanes t = 2 (run & 1) and the next, as their columns 16 e + 4 t..
-                uint8_t* dst = xs + (run >> 2) * (kPlanes * plane_bytes) +
-                               ((run & 1) * 2 * tokens + token) * kRunBytes + (run >> 1 & 1) * (kRunBytes / 2);
+                uint32_t r[kTogether][kPlanes][kRunBytes / 4];
 #pragma unroll
-                for (int pl = 0; pl < kPlanes; ++pl) {
-                    uint8_t* d = dst + pl * plane_bytes;
-                    if constexpr (KIND == kI8) {  // the codes' byte order: 0, 2, 1, 3
-                        *reinterpret_cast<uint32_t*>(d) = __byte_perm(r[0][0], 0, 0x3120);
-                        *reinterpret_cast<uint32_t*>(d + tokens * kRunBytes) = __byte_perm(r[0][1], 0, 0x3120);
-                    } else {
-                        *reinterpret_cast<uint2*>(d) = make_uint2(r[pl][0], r[pl][1]);
-                        *reinterpret_cast<uint2*>(d + tokens * kRunBytes) = make_uint2(r[pl][2], r[pl][3]);
+                for (int i = 0; i < kTogether; ++i) {
+                    const int token = min(first_token + i, tokens - 1);
+                    const uint8_t* row = static_cast<const uint8_t*>(p.x) + (token0 + token) * p.x_stride * x_size;
+                    load_run<KIND>(p, row, (begin + from) * kChunk + run * 8, p.k, r[i]);
+                }
+                // The run's two quads go to lanes t = 2 (run & 1) and the next, as their columns 16 e + 4 t..
+#pragma unroll
+                for (int i = 0; i < kTogether; ++i) {
+                    const int token = min(first_token + i, tokens - 1);
+                    uint8_t* dst = xs + (run >> 2) * (kPlanes * plane_bytes) +
+                                   ((run & 1) * 2 * tokens + token) * kRunBytes + (run >> 1 & 1) * (kRunBytes / 2);
+#pragma unroll
+                    for (int pl = 0; pl < kPlanes; ++pl) {
+                        uint8_t* d = dst + pl * plane_bytes;
+                        if constexpr (KIND == kI8) {  // the codes' byte order: 0, 2, 1, 3
+                            *reinterpret_cast<uint32_t*>(d) = __byte_perm(r[i][0][0], 0, 0x3120);
+                            *reinterpret_cast<uint32_t*>(d + tokens * kRunBytes) = __byte_perm(r[i][0][1], 0, 0x3120);
+                        } else {
+                            *reinterpret_cast<uint2*>(d) = make_uint2(r[i][pl][0], r[i][pl][1]);
+                            *reinterpret_cast<uint2*>(d + tokens * kRunBytes) = make_uint2(r[i][pl][2], r[i][pl][3]);
+                        }
                     }
                 }
             }
         }
     };
+    const auto stage_x = [&](int from) {
+        const int runs = min(p.x_chunks, end - begin - from) * 16;  // runs of eight of a token: chunk, h, t
+        // The loads of all tokens (of four, for fp32) are under way before the first is stored.
+        if (tokens == 1) stage(std::integral_constant<int, 1>(), from, runs);
+        else if (tokens == 2) stage(std::integral_constant<int, 2>(), from, runs);
+        else if (tokens <= 4 || kPlanes == 3) stage(std::integral_constant<int, 4>(), from, runs);
+        else stage(std::integral_constant<int, 8>(), from, runs);
+    };
 
-    float acc[4][NB][4];
+    float acc[4][4];
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[r][b][e] = 0.0f;
+        for (int e = 0; e < 4; ++e) acc[r][e] = 0.0f;
 
     // A lane of a token beyond the last reads the last: its column of the product is never stored.
-    const uint32_t x_lane = mv::smem_addr(xs) + t * tokens * kRunBytes;
-    uint32_t x_token[NB];
-#pragma unroll
-    for (int b = 0; b < NB; ++b) x_token[b] = min(8 * b + g, tokens - 1) * kRunBytes;
+    const uint32_t x_lane = mv::smem_addr(xs) + (t * tokens + min(g, tokens - 1)) * kRunBytes;
     int drain = 0;  // stage of the record that is read next
     for (int from = 0; from < end - begin; from += p.x_chunks) {
     if (from) __syncthreads();  // every warp is done with the chunks of x before
@@ -430,15 +444,13 @@ __global__ void __launch_bounds__(kThreads, NB == 4 ? 2 : 4) w4_linear_kernel(co
                 // Sums start at 1.5 2^23 as a float's bits: their float value is then one subtraction away,
                 // as they stay below 2^22 (16 * 8 * 128 * 128, or 15 * 128 * 128 with zero points).
                 constexpr int kBias = 0x4b400000;
-                int c[2][NB][4];
+                int c[2][4];
                 uint32_t zl[2], zh[2];
 #pragma unroll
                 for (int h = 0; h < 4; ++h) {
                     if (h % kGroupRuns == 0) {
 #pragma unroll
-                        for (int b = 0; b < NB; ++b)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) c[0][b][e] = c[1][b][e] = kBias;
+                        for (int e = 0; e < 4; ++e) c[0][e] = c[1][e] = kBias;
                         if constexpr (ZEROS) {
                             // zero - 8 as a byte, plus 8, in all four bytes of an operand.
                             const uint32_t z = lds32(zeros + (h / kGroupRuns) * 64 + rp * 4) ^ 0x88888888u;
@@ -463,29 +475,23 @@ __global__ void __launch_bounds__(kThreads, NB == 4 ? 2 : 4) w4_linear_kernel(co
                         a1[0] = (w.z << 4) & 0xf0f0f0f0u, a1[1] = w.z & 0xf0f0f0f0u;
                         a1[2] = (w.w << 4) & 0xf0f0f0f0u, a1[3] = w.w & 0xf0f0f0f0u;
                     }
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        const uint2 xv = lds64(x_chunk + h * plane_bytes + x_token[b]);
-                        mma_s8(c[0][b], a0, xv.x, xv.y);
-                        mma_s8(c[1][b], a1, xv.x, xv.y);
-                    }
+                    const uint2 xv = lds64(x_chunk + h * plane_bytes);
+                    mma_s8(c[0], a0, xv.x, xv.y);
+                    mma_s8(c[1], a1, xv.x, xv.y);
                     if (h % kGroupRuns == kGroupRuns - 1) {
                         const uint2 s = lds64(scales + (h / kGroupRuns) * 128 + rp * 8);
 #pragma unroll
                         for (int q = 0; q < 2; ++q) {
                             const float2 sc = scale_pair(q ? s.y : s.x, p.scale_bf16);
 #pragma unroll
-                            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                                for (int e = 0; e < 4; ++e)
-                                    acc[2 * rp + q][b][e] =
-                                        fmaf(e < 2 ? sc.x : sc.y, __int_as_float(c[q][b][e]) - 12582912.0f,
-                                             acc[2 * rp + q][b][e]);
+                            for (int e = 0; e < 4; ++e)
+                                acc[2 * rp + q][e] = fmaf(e < 2 ? sc.x : sc.y, __int_as_float(c[q][e]) - 12582912.0f,
+                                                          acc[2 * rp + q][e]);
                         }
                     }
                 }
             } else {
-                float c[2][NB][4];
+                float c[2][4];
                 uint32_t zl[2], zh[2];
 #pragma unroll
                 for (int h = 0; h < 4; ++h) {
@@ -498,13 +504,9 @@ __global__ void __launch_bounds__(kThreads, NB == 4 ? 2 : 4) w4_linear_kernel(co
                             zh[q] = A::zero_high(8 + static_cast<int8_t>(z >> (16 * q + 8)));
                         }
                     }
-                    uint4 xv[NB][kPlanes];
+                    uint4 xv[kPlanes];
 #pragma unroll
-                    for (int b = 0; b < NB; ++b)
-#pragma unroll
-                        for (int pl = 0; pl < kPlanes; ++pl) {
-                            xv[b][pl] = lds128(x_chunk + (h * kPlanes + pl) * plane_bytes + x_token[b]);
-                        }
+                    for (int pl = 0; pl < kPlanes; ++pl) xv[pl] = lds128(x_chunk + (h * kPlanes + pl) * plane_bytes);
                     const uint4 w = lds128(rec + ((h * 2 + rp) * 32 + lane) * 16);
                     const uint32_t words[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -512,14 +514,11 @@ __global__ void __launch_bounds__(kThreads, NB == 4 ? 2 : 4) w4_linear_kernel(co
                         uint32_t a[4];
                         A::weights(words[j], zl[j >> 1], zh[j >> 1], a);
 #pragma unroll
-                        for (int b = 0; b < NB; ++b)
-#pragma unroll
-                            for (int pl = 0; pl < kPlanes; ++pl) {
-                                const uint32_t b0 = j & 1 ? xv[b][pl].z : xv[b][pl].x;
-                                const uint32_t b1 = j & 1 ? xv[b][pl].w : xv[b][pl].y;
-                                if (h % kGroupRuns == 0 && (j & 1) == 0 && pl == 0) A::mma_first(c[j >> 1][b], a, b0, b1);
-                                else A::mma(c[j >> 1][b], a, b0, b1);
-                            }
+                        for (int pl = 0; pl < kPlanes; ++pl) {
+                            const uint32_t b0 = j & 1 ? xv[pl].z : xv[pl].x, b1 = j & 1 ? xv[pl].w : xv[pl].y;
+                            if (h % kGroupRuns == 0 && (j & 1) == 0 && pl == 0) A::mma_first(c[j >> 1], a, b0, b1);
+                            else A::mma(c[j >> 1], a, b0, b1);
+                        }
                     }
                     if (h % kGroupRuns == kGroupRuns - 1) {
                         const uint2 s = lds64(scales + (h / kGroupRuns) * 128 + rp * 8);
@@ -527,11 +526,8 @@ __global__ void __launch_bounds__(kThreads, NB == 4 ? 2 : 4) w4_linear_kernel(co
                         for (int q = 0; q < 2; ++q) {
                             const float2 sc = scale_pair(q ? s.y : s.x, p.scale_bf16);
 #pragma unroll
-                            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                                for (int e = 0; e < 4; ++e)
-                                    acc[2 * rp + q][b][e] =
-                                        fmaf(e < 2 ? sc.x : sc.y, c[q][b][e], acc[2 * rp + q][b][e]);
+                            for (int e = 0; e < 4; ++e)
+                                acc[2 * rp + q][e] = fmaf(e < 2 ? sc.x : sc.y, c[q][e], acc[2 * rp + q][e]);
                         }
                     }
                 }
@@ -548,15 +544,13 @@ __global__ void __launch_bounds__(kThreads, NB == 4 ? 2 : 4) w4_linear_kernel(co
     {
         float* part = reinterpret_cast<float*>(smem + warp * p.ring_bytes);
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                float* at = part + (8 * b + 2 * t) * kPartStride + 16 * r + g;
-                at[0] = acc[r][b][0];
-                at[kPartStride] = acc[r][b][1];
-                at[8] = acc[r][b][2];
-                at[kPartStride + 8] = acc[r][b][3];
-            }
+        for (int r = 0; r < 4; ++r) {
+            float* at = part + 2 * t * kPartStride + 16 * r + g;
+            at[0] = acc[r][0];
+            at[kPartStride] = acc[r][1];
+            at[8] = acc[r][2];
+            at[kPartStride + 8] = acc[r][3];
+        }
     }
     __syncthreads();
     const int tiles_here = kWarps / p.ksplit;
