@@ -196,9 +196,10 @@ int mvq_w4_linear(const MvqLinearArgs* a, void* stream) try {
     p.out = a->out;
     p.out_stride = a->out_stride_row;
     p.out_dtype = static_cast<int>(a->out_dtype);
-    p.x_units = a->x_dtype == MVQ_DTYPE_I8 ? p.x_runs && a->k % 16 == 0 && address(a->x) % 16 == 0 &&
-                                                 (a->m == 1 || a->x_stride_row % 16 == 0)
-                                           : p.x_runs && size == 2;
+    // TMA wants 16-byte rows that do not overlap.
+    p.x_units = (size == 2 || a->x_dtype == MVQ_DTYPE_I8) && address(a->x) % 16 == 0 &&
+                (a->m == 1 || (a->x_stride_row * size % 16 == 0 && a->x_stride_row >= a->k &&
+                               a->x_stride_row < (int64_t(1) << 38)));
     const int kind = a->x_dtype == MVQ_DTYPE_E4M3 ? mvq::kF16 : static_cast<int>(a->x_dtype);
     const int group = static_cast<int>(a->group);
     int few = 8;

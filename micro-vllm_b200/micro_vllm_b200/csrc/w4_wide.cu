@@ -1,6 +1,8 @@
 // Plans and launches of the tcgen05 product kernel (w4_wide.cuh), and the device status that its waits set.
 #include <algorithm>
 #include <cstdlib>
+#include <cudaTypedefs.h>
+
 #include <mutex>
 
 #include "mvq_host.cuh"
@@ -9,21 +11,52 @@
 namespace mvq {
 namespace {
 
-// CTAs that share a block of rows' columns: the number in 1..8 that fills whole
-// rounds of the SMs best.
-int wide_cluster(int64_t blocks, int chunks, int sms) {
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* ptr = nullptr;
+        cudaDriverEntryPointQueryResult status;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &status) == cudaSuccess &&
+            status == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+    });
+    return fn;
+}
+
+// X as [m, k] in boxes of `rows` rows of 128 bytes, swizzled; what lies beyond reads as zero.
+int x_map(const LinearParams& p, int kind, int rows, CUtensorMap* map) {
+    auto encode = encode_fn();
+    if (!encode) return fail(MVQ_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable from the driver");
+    const int size = kind == kI8 ? 1 : 2;
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(p.k), static_cast<cuuint64_t>(p.m)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(p.m == 1 ? (p.k * size + 15) / 16 * 16 : p.x_stride * size)};
+    const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / size), static_cast<cuuint32_t>(rows)};
+    const cuuint32_t steps[2] = {1, 1};
+    const CUresult r = encode(map, kind == kI8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                   : kind == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                              2, const_cast<void*>(p.x), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(MVQ_ERR_CUDA, "cuTensorMapEncodeTiled failed (CUresult %d)", static_cast<int>(r));
+    return MVQ_OK;
+}
+
+// CTAs that share a block of rows' columns: the number in 1..8 with the least
+// estimated time. An SM takes its share of the CTAs; each costs `start` and its
+// chunks. WIDE_NOTE
+int wide_cluster(int64_t blocks, int chunks, int sms, int nt) {
 #ifdef MVQ_TUNE
     if (getenv("CL")) return atoi(getenv("CL"));
 #endif
+    const double start = nt <= 32 ? 4.0 : nt == 64 ? 6.5 : 9.0;
+    const double chunk = nt == 16 ? 0.3 : nt == 32 ? 0.33 : nt == 64 ? 0.59 : 0.75;
     int best = 1;
-    double most = 0.0;
+    double least = 0.0;
     for (int c = 1; c <= 8 && c <= chunks; ++c) {
-        const int64_t ctas = blocks * c;
-        const int64_t rounds = (ctas + sms - 1) / sms;
-        // The longest run of chunks, in each of the rounds.
-        const double used = static_cast<double>(blocks) * chunks /
-                            (static_cast<double>(rounds) * sms * ((chunks + c - 1) / c));
-        if (used > most * 1.02) most = used, best = c;
+        const int64_t per_sm = (blocks * c + sms - 1) / sms;
+        const double time = static_cast<double>(per_sm) * (start + chunk * ((chunks + c - 1) / c));
+        if (c == 1 || time < least) least = time, best = c;
     }
     return best;
 }
@@ -50,9 +83,14 @@ int launch_one(LinearParams p, int device, int sms, void* stream) {
     const int64_t blocks = (static_cast<int64_t>(p.n) + kWideRows - 1) / kWideRows;
     const int64_t passes = (static_cast<int64_t>(p.m) + NT - 1) / NT;
     if (passes > 65535) return fail(MVQ_ERR_UNSUPPORTED, "too many rows of x for one call");
-    p.cluster = wide_cluster(blocks * passes, p.chunks, sms);
+    p.cluster = wide_cluster(blocks * passes, p.chunks, sms, NT);
+    CUtensorMap map = {};
+    if (p.x_units) {
+        const int rc = x_map(p, KIND, NT, &map);
+        if (rc != MVQ_OK) return rc;
+    }
     const dim3 grid(static_cast<unsigned>(blocks * p.cluster), static_cast<unsigned>(passes));
-    const cudaError_t err = launch(kernel, grid, Shape::kThreads, kSmem, p.cluster, stream, p);
+    const cudaError_t err = launch(kernel, grid, Shape::kThreads, kSmem, p.cluster, stream, p, map);
     return err == cudaSuccess ? MVQ_OK : cuda_fail(err, "wide 4-bit linear kernel launch");
 }
 

@@ -19,12 +19,12 @@
 // twice the bandwidth that is left).
 //
 // Warps: 0-7 convert, two sets of four taking chunks in turn (warp w fills lanes
-// 32 (w % 4).. of A); then sets of four that load X (cp.async, three chunks ahead)
-// and drain 32 columns of D each; the last issues the MMAs. A wait that finds its
-// barrier complete still costs some 200 cycles, as does a commit, so there are few
-// of them, and two sets convert so that one's waits hide behind the other. Every
-// wait is bounded (2 s): one that gives up sets the device status, and the CTA's
-// results are NaN.
+// 32 (w % 4).. of A); then sets of four that drain 32 columns of D each; one that
+// issues the MMAs; one that issues X's TMA loads. A wait that finds its barrier
+// complete still costs some 200 cycles, as does a commit, so there is one barrier
+// for all that a chunk's MMAs need and one for their end, and two sets convert so
+// that one's waits hide behind the other. Every wait is bounded (2 s): one that
+// gives up sets the device status, and the CTA's results are NaN.
 #pragma once
 
 #include "w4_linear.cuh"
@@ -32,7 +32,6 @@
 namespace mvq {
 
 constexpr int kWideRows = 128;
-constexpr int kWideXBuffers = 4;
 constexpr int kWidePartStride = 132;  // floats per token of the partial sums [token][128 rows]
 
 template <int KIND, int NT, int GROUP, bool ZEROS>
@@ -40,19 +39,19 @@ struct WideShape {
     static constexpr int kGroups = kChunk / GROUP;
     static constexpr int kCols = NT < 32 ? NT : 32;        // columns of D that a set drains
     static constexpr int kSets = NT / kCols;
-    static constexpr int kThreads = (8 + 4 * kSets + 1) * 32;
+    static constexpr int kTurns = NT == 64 ? 2 : 1;        // groups of sets that take chunks in turn (NT 128 leaves no threads for it)
+    static constexpr int kThreads = (8 + 4 * kSets * kTurns + 2) * 32;
     static constexpr int kCtas = NT <= 32 ? 2 : 1;         // per SM
     static constexpr int kStages = NT == 64 ? 5 : 3;       // records in flight per converting warp
     static constexpr int kACols = KIND == kI8 ? 32 : 64;   // TMEM columns of a chunk of A
-    static constexpr int kABuffers = NT <= 32 && KIND != kI8 ? 3 : 4;
+    static constexpr int kBuffers = NT <= 32 && KIND != kI8 ? 3 : 4;  // chunks of A and of X
     static constexpr int kTmemCols = NT <= 32 ? 256 : 512;
-    static_assert(kABuffers * kACols + 2 * NT <= kTmemCols, "TMEM columns");
+    static_assert(kBuffers * kACols + 2 * NT <= kTmemCols, "TMEM columns");
     static constexpr int kXBytes = NT * (KIND == kI8 ? 128 : 256);
     static constexpr int kStageBytes = kCodeBytes / 2 + (ZEROS ? kGroups * 64 : 0);
-    static constexpr int kScaleBytes = kSets * kGroups * 128 * 4;  // per chunk: a word for each draining thread
     static constexpr int kRings = 8 * kStages * kStageBytes;
-    static constexpr int kUsed = kWideXBuffers * (kXBytes + kScaleBytes) + kRings;
-    static constexpr int kPart = NT * kWidePartStride * 4;
+    static constexpr int kUsed = kBuffers * kXBytes + kRings;
+    static constexpr int kPart = kTurns * NT * kWidePartStride * 4;
     static constexpr int kSmem = (kUsed > kPart ? kUsed : kPart) + 1024;
 };
 
@@ -62,10 +61,10 @@ __device__ __forceinline__ uint64_t sw128_desc(uint32_t addr) {
            (static_cast<uint64_t>(2) << 61);
 }
 
-__device__ __forceinline__ bool elect_one() {
+__device__ __forceinline__ uint32_t elect_one() {
     uint32_t leader;
     asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(leader));
-    return leader != 0;
+    return leader;
 }
 
 // D fp32 (1) or s32 (2); A and B fp16 (0), bf16 (1) or s8 (1); both K-major.
@@ -75,22 +74,52 @@ __host__ __device__ constexpr uint32_t wide_idesc() {
            (static_cast<uint32_t>(NT >> 3) << 17) | (static_cast<uint32_t>(kWideRows >> 4) << 24);
 }
 
+// Issued by the lane with `leader` set, in code that the whole warp runs: the
+// operands then stay in uniform registers. (In a branch of one lane each MMA took
+// some 60 cycles to issue, for moving them there.)
 template <int KIND>
-__device__ __forceinline__ void wide_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+__device__ __forceinline__ void wide_mma(uint32_t leader, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
     if constexpr (KIND == kI8)
         asm volatile(
-            "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-            " tcgen05.mma.cta_group::1.kind::i8 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-            "r"(a), "l"(b), "r"(idesc), "r"(add));
+            "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+            " @q tcgen05.mma.cta_group::1.kind::i8 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+            "r"(a), "l"(b), "r"(idesc), "r"(add), "r"(leader));
     else
         asm volatile(
-            "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-            " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-            "r"(a), "l"(b), "r"(idesc), "r"(add));
+            "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+            " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+            "r"(a), "l"(b), "r"(idesc), "r"(add), "r"(leader));
 }
 
-__device__ __forceinline__ void wide_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+__device__ __forceinline__ void wide_commit(uint32_t leader, uint32_t bar) {
+    asm volatile(
+        "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+        " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar),
+        "r"(leader)
+        : "memory");
+}
+
+// As mv::mbar_wait_bounded, with each try suspended for up to 20 us: many warps
+// wait here, and tries that come back at once take issue slots from those that
+// convert.
+__device__ __forceinline__ bool wide_try(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(done)
+        : "r"(bar), "r"(parity), "r"(20000)
+        : "memory");
+    return done != 0;
+}
+__device__ __forceinline__ bool wide_wait(uint32_t bar, uint32_t parity) {
+    if (wide_try(bar, parity)) return true;
+    const unsigned long long start = mv::global_timer_ns();
+    while (true) {
+#pragma unroll 1
+        for (int i = 0; i < 16; ++i)
+            if (wide_try(bar, parity)) return true;
+        if (mv::global_timer_ns() - start > mv::kWaitLimitNs) return false;
+    }
 }
 __device__ __forceinline__ void wide_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -120,31 +149,34 @@ __device__ __forceinline__ void tmem_ld_16(uint32_t taddr, uint32_t (&r)[16]) {
         : "r"(taddr));
 }
 
-__device__ __forceinline__ void cp_async_16_or_zero(uint32_t dst, const void* src, bool real) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+            dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+        : "memory");
 }
 
+// `xmap`: X as [m, k] in boxes of NT rows of 128 bytes, where p.x_units says that it can be copied as it is.
 template <int KIND, int NT, int GROUP, bool ZEROS>
 __global__ void __launch_bounds__(WideShape<KIND, NT, GROUP, ZEROS>::kThreads, WideShape<KIND, NT, GROUP, ZEROS>::kCtas)
-w4_wide_kernel(const LinearParams p) {
+w4_wide_kernel(const LinearParams p, const __grid_constant__ CUtensorMap xmap) {
     using A = Act<KIND>;
     using Shape = WideShape<KIND, NT, GROUP, ZEROS>;
     constexpr int kGroups = Shape::kGroups;
     constexpr int kRecord = record_size(GROUP, ZEROS);
-    constexpr int kStages = Shape::kStages, kAB = Shape::kABuffers, kSets = Shape::kSets;
-    constexpr int kMmaWarp = 8 + 4 * kSets;
+    constexpr int kStages = Shape::kStages, kAB = Shape::kBuffers, kSets = Shape::kSets;
+    constexpr int kTurns = Shape::kTurns, kMmaWarp = 8 + 4 * kSets * kTurns, kLoadWarp = kMmaWarp + 1;
     extern __shared__ uint8_t smem_raw[];
-    // Per chunk one barrier for both operands (full) and one for the end of its
-    // last group (done, which frees A and X and hands over D); part_done and
-    // d_empty only serve chunks of several groups.
+    // full: a chunk's A and X are in place and D of the chunk two before is
+    // drained. done: its last group is multiplied, which frees A and X and hands
+    // over D. part_done and d_empty only serve chunks of several groups.
     __shared__ __align__(8) uint64_t full[kAB], done[kAB], part_done[2], d_empty[2], drained;
     __shared__ uint32_t s_tmem;
+    __shared__ float s_scale[NT], s_bias[kWideRows];
     __shared__ volatile int s_failed;
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int rank = p.cluster > 1 ? static_cast<int>(cluster_rank()) : 0;
     const int64_t block = static_cast<int64_t>(blockIdx.x) / p.cluster;  // of 128 weight rows
     const int token0 = blockIdx.y * NT;
@@ -155,8 +187,7 @@ w4_wide_kernel(const LinearParams p) {
     uint8_t* const smem =
         reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     const uint32_t xs = mv::smem_addr(smem);
-    const uint32_t scale_at = xs + kWideXBuffers * Shape::kXBytes;
-    const uint32_t rings = scale_at + kWideXBuffers * Shape::kScaleBytes;
+    const uint32_t rings = xs + kAB * Shape::kXBytes;
 
     // A converting or draining warp w has rows 32 (w % 4).. of the 128: half p = w & 1
     // of tile (w % 4) >> 1. A second tile beyond the weight's last reads the
@@ -166,11 +197,11 @@ w4_wide_kernel(const LinearParams p) {
     const uint8_t* const records = p.records + (tile * p.chunks + begin) * static_cast<int64_t>(kRecord);
     const uint8_t* const codes = records + (quarter & 1) * 512 + lane * 16;
     const uint32_t ring = rings + (warp & 7) * kStages * Shape::kStageBytes;
-    const int set = warp < 8 ? warp >> 2 : (warp - 8) >> 2;
+    const int set = warp < 8 ? warp >> 2 : ((warp - 8) >> 2) % kSets;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kAB; ++i) {
-            mv::mbar_init(mv::smem_addr(&full[i]), 4 + 4 * kSets);  // a converting set and all loading warps
+            mv::mbar_init(mv::smem_addr(&full[i]), 4 + 4 * kSets + 1);  // a converting set, the sets that drain a chunk, the loader
             mv::mbar_init(mv::smem_addr(&done[i]), 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -212,10 +243,10 @@ w4_wide_kernel(const LinearParams p) {
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tmem = s_tmem;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);  // the same in every lane, for the compiler too
     const uint32_t d_col = tmem + kAB * Shape::kACols;
     const auto wait = [&](uint64_t* bar, int parity) {  // of a whole warp
-        const bool ok = __all_sync(0xffffffffu, mv::mbar_wait_bounded(mv::smem_addr(bar), parity & 1));
+        const bool ok = __all_sync(0xffffffffu, wide_wait(mv::smem_addr(bar), parity & 1));
         if (!ok) {
             s_failed = 1;
             if (lane == 0) atomicOr(&mv::g_device_status, mv::kStatusWaitTimeout);
@@ -283,126 +314,137 @@ w4_wide_kernel(const LinearParams p) {
                     }
                 }
             }
-            if (ZEROS) __syncwarp();
-            issue_codes(i + 2 * kStages);
             wait_st();
             fence_before();
             __syncwarp();
             if (lane == 0) wide_arrive(mv::smem_addr(&full[i % kAB]));
+            issue_codes(i + 2 * kStages);
         }
         cp_async_wait<0>();
     } else if (warp == kMmaWarp) {
-        // The whole warp runs the loop, so that the operands' addresses are
-        // uniform; one elected lane issues.
         constexpr int kSteps = KIND == kI8 ? GROUP / 32 : GROUP / 16;  // MMAs per group
-        const bool leader = elect_one();
+        const uint32_t leader = elect_one();
         bool ok = true;
-        for (int i = 0; i < n && ok; ++i) {
+        for (int i = 0; i < n; ++i) {
             ok = wait(&full[i % kAB], i / kAB);
 #pragma unroll
             for (int gi = 0; gi < kGroups; ++gi) {
                 const int u = i * kGroups + gi;
-                // With one group the loading warps' arrival for chunk i says that D of chunk i - 2 is drained.
                 if (kGroups > 1 && u >= 2) ok = ok && wait(&d_empty[u & 1], (u >> 1) - 1);
+                if (!ok) break;
                 fence_after();
-                if (leader && ok) {
-                    const uint32_t a_at = tmem + (i % kAB) * Shape::kACols + gi * kSteps * 8;
-                    const uint32_t x_at = xs + (i % kWideXBuffers) * Shape::kXBytes;
+                const uint32_t a_at = tmem + (i % kAB) * Shape::kACols + gi * kSteps * 8;
+                const uint32_t x_at = xs + (i % kAB) * Shape::kXBytes;
 #pragma unroll
-                    for (int s = 0; s < kSteps; ++s) {
-                        const int step = gi * kSteps + s;
-                        const uint32_t b = KIND == kI8 ? x_at + step * 32 : x_at + (step >> 2) * (NT * 128) + (step & 3) * 32;
-                        wide_mma<KIND>(d_col + (u & 1) * NT, a_at + s * 8, sw128_desc(b), wide_idesc<KIND, NT>(), s > 0);
-                    }
-                    wide_commit(mv::smem_addr(gi == kGroups - 1 ? &done[i % kAB] : &part_done[(i * (kGroups - 1) + gi) & 1]));
+                for (int s = 0; s < kSteps; ++s) {
+                    const int step = gi * kSteps + s;
+                    const uint32_t b = KIND == kI8 ? x_at + step * 32 : x_at + (step >> 2) * (NT * 128) + (step & 3) * 32;
+                    wide_mma<KIND>(leader, d_col + (u & 1) * NT, a_at + s * 8, sw128_desc(b), wide_idesc<KIND, NT>(), s > 0);
                 }
-                __syncwarp();
+                wide_commit(leader, mv::smem_addr(gi == kGroups - 1 ? &done[i % kAB]
+                                                                    : &part_done[(i * (kGroups - 1) + gi) & 1]));
             }
+            if (!ok) break;
         }
         // Everything issued completes before TMEM is freed.
-        if (leader) wide_commit(mv::smem_addr(&drained));
-        __syncwarp();
+        wide_commit(leader, mv::smem_addr(&drained));
         wait(&drained, 0);
+    } else if (warp == kLoadWarp) {
+        const uint32_t leader = elect_one();
+        bool ok = true;
+        for (int i = 0; i < n && ok; ++i) {
+            if (i >= kAB) ok = wait(&done[i % kAB], i / kAB - 1);
+            if (leader && ok) {
+                const uint32_t bar = mv::smem_addr(&full[i % kAB]);
+                if (p.x_units) {
+                    mv::mbar_arrive_expect_tx(bar, Shape::kXBytes);
+                    const uint32_t dst = xs + (i % kAB) * Shape::kXBytes;
+                    const int k = (begin + i) * kChunk;
+                    tma_load_2d(dst, &xmap, k, token0, bar);
+                    if (KIND != kI8) tma_load_2d(dst + NT * 128, &xmap, k + 64, token0, bar);
+                } else {
+                    wide_arrive(bar);  // the draining warps store X themselves
+                }
+            }
+            __syncwarp();
+        }
+        // What the epilogue needs of every token and row.
+        for (int t = lane; t < NT; t += 32)
+            s_scale[t] = (ZEROS && KIND == kI8 ? 1.0f : A::kScale) * (p.x_scale && t < tokens ? p.x_scale[token0 + t] : 1.0f);
+        for (int r = lane; r < kWideRows; r += 32) {
+            const int64_t column = block * kWideRows + r;
+            s_bias[r] = p.bias && column < p.n ? load_as_float(p.bias, column, p.out_dtype) : 0.0f;
+        }
+        // A wait gave up: no barrier tells any more when the copies under way land, so give them their time.
+        if (!ok)
+            for (int i = 0; i < 1000; ++i) __nanosleep(1000);
     } else {
-        constexpr int kLoaders = 128 * kSets;
-        const int lt = threadIdx.x - 256;
-        constexpr int kUnits = KIND == kI8 ? 8 : 16;  // 16-byte units of a token's chunk
-        constexpr int kTurns = NT * kUnits / kLoaders;
-        constexpr int kTokens = kLoaders / kUnits;    // tokens of a turn
-        const int x_size = p.x_dtype == kF32 ? 4 : p.x_dtype >= kI8 ? 1 : 2;
+        constexpr int kDrainers = 128 * kSets;
+        const int turn = (warp - 8) / (4 * kSets);
+        const int lt = threadIdx.x - 256 - turn * kDrainers;
         // This thread's scale: row `lane` of the quarter, its pair of rows g and g + 8 in a word.
         const uint8_t* const scale = records + kCodeBytes + ((lane & 7) * 8 + (quarter & 1) * 4 + (lane >> 4) * 2) * 2;
-        // This thread's units: `unit` of tokens first, first + kTokens, ... (all at one place of the swizzle).
-        const int first = lt / kUnits, unit = lt % kUnits;
-        const uint32_t unit_at = (unit >> 3) * (NT * 128) + first * 128 + (((unit & 7) ^ (first & 7)) << 4);
-        const uint8_t* const rows = static_cast<const uint8_t*>(p.x) + (token0 + first) * p.x_stride * x_size;
-        const int64_t row_step = kTokens * p.x_stride * x_size;
-        const auto issue_x = [&](int i) {
-            if (lane < kGroups && i + 2 < n)  // the scales come from memory: into L2 before they are copied
-                asm volatile("prefetch.global.L2 [%0];" ::"l"(records + static_cast<int64_t>(i + 2) * kRecord + kCodeBytes + lane * 128));
-            if (i < n) {
-                const uint32_t dst = xs + (i % kWideXBuffers) * Shape::kXBytes + unit_at;
-                const int k = (begin + i) * kChunk + unit * (KIND == kI8 ? 16 : 8);
-                if (p.x_units) {
+        const auto load_scales = [&](int i, uint32_t (&w)[kGroups]) {
 #pragma unroll
-                    for (int j = 0; j < kTurns; ++j) {
-                        const bool real = first + j * kTokens < tokens && k < p.k;
-                        cp_async_16_or_zero(dst + j * kTokens * 128,
-                                            real ? rows + j * row_step + k * x_size : static_cast<const uint8_t*>(p.x), real);
-                    }
-                } else {  // a loop, and apart from the other: what warps of several roles run has to fit the instruction cache
+            for (int gi = 0; gi < kGroups; ++gi)
+                if (i < n)
+                    w[gi] = __ldg(reinterpret_cast<const uint32_t*>(scale + static_cast<int64_t>(i) * kRecord + gi * 128));
+        };
+        // X that TMA cannot copy as it is (rows off a 16-byte boundary, e4m3 numbers
+        // that become fp16): these warps store it, element by element at worst.
+        const auto store_x = [&](int i) {
+            constexpr int kUnits = KIND == kI8 ? 8 : 16;  // 16-byte units of a token's chunk
+            const int x_size = p.x_dtype >= kI8 ? 1 : 2;
+            const uint32_t dst = xs + (i % kAB) * Shape::kXBytes;
 #pragma unroll 1
-                    for (int j = 0; j < kTurns; ++j) {
-                        const int limit = first + j * kTokens < tokens ? p.k : 0;
-                        uint32_t r[1][A::kRunBytes / 4];
-                        uint4 v;
-                        load_run<KIND>(p, rows + j * row_step, k, limit, r);
-                        if constexpr (KIND == kI8) {
-                            v.x = r[0][0], v.y = r[0][1];
-                            load_run<KIND>(p, rows + j * row_step, k + 8, limit, r);
-                            v.z = r[0][0], v.w = r[0][1];
-                        } else {
-                            v = make_uint4(r[0][0], r[0][1], r[0][2], r[0][3]);
-                        }
-                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + j * kTokens * 128),
-                                     "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
-                                     : "memory");
-                    }
+            for (int u = lt; u < NT * kUnits; u += kDrainers) {
+                const int token = u / kUnits, unit = u % kUnits;
+                const int limit = token < tokens ? p.k : 0;
+                const int k = (begin + i) * kChunk + unit * (KIND == kI8 ? 16 : 8);
+                const uint8_t* row = static_cast<const uint8_t*>(p.x) + (token0 + token) * p.x_stride * x_size;
+                uint32_t r[1][A::kRunBytes / 4];
+                uint4 v;
+                load_run<KIND>(p, row, k, limit, r);
+                if constexpr (KIND == kI8) {
+                    v.x = r[0][0], v.y = r[0][1];
+                    load_run<KIND>(p, row, k + 8, limit, r);
+                    v.z = r[0][0], v.w = r[0][1];
+                } else {
+                    v = make_uint4(r[0][0], r[0][1], r[0][2], r[0][3]);
                 }
-#pragma unroll
-                for (int gi = 0; gi < kGroups; ++gi)
-                    cp_async_4(scale_at + (i % kWideXBuffers) * Shape::kScaleBytes + (gi * kLoaders + lt) * 4,
-                               scale + static_cast<int64_t>(i) * kRecord + gi * 128);
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(
+                                 dst + (unit >> 3) * (NT * 128) + token * 128 + (((unit & 7) ^ (token & 7)) << 4)),
+                             "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                             : "memory");
             }
-            cp_async_commit();
+            mv::fence_proxy_async_smem();
         };
         float acc[Shape::kCols];
 #pragma unroll
         for (int e = 0; e < Shape::kCols; ++e) acc[e] = 0.0f;
         const uint32_t lanes = d_col + set * Shape::kCols + (static_cast<uint32_t>(quarter * 32) << 16);
-        const auto publish = [&](int i) {  // chunk i of X is in shared memory, D of chunk i - 2 in registers
+        const auto publish = [&](int i) {  // chunk i may be multiplied, as far as these warps go
             if (i >= n) return;
-            mv::fence_proxy_async_smem();
+            if (!p.x_units) store_x(i);
             fence_before();
             __syncwarp();
             if (lane == 0) wide_arrive(mv::smem_addr(&full[i % kAB]));
         };
-        for (int i = 0; i < kWideXBuffers - 1; ++i) issue_x(i);
-        cp_async_wait<kWideXBuffers - 2>();
-        publish(0);
+        uint32_t scales[kGroups] = {}, scales1[kGroups] = {}, scales2[kGroups] = {};
+        load_scales(turn, scales);
+        load_scales(turn + kTurns, scales1);
+        publish(turn);
+        if (kTurns == 1) publish(1);
         bool ok = true;
-        for (int i = 0; i < n && ok; ++i) {
+        for (int i = turn; i < n && ok; i += kTurns) {
+            load_scales(i + 2 * kTurns, scales2);
+            if (lane < kGroups && i + 6 < n)  // the scales come from memory: into L2 well before
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(records + static_cast<int64_t>(i + 6) * kRecord + kCodeBytes +
+                                                             lane * 128));
 #pragma unroll
             for (int gi = 0; gi < kGroups; ++gi) {
-                if (gi == 0) {
-                    // Chunk i + kWideXBuffers - 1 goes where chunk i - 1 was, whose D this warp has drained.
-                    issue_x(i + kWideXBuffers - 1);
-                    cp_async_wait<kWideXBuffers - 2>();
-                    publish(i + 1);
-                }
                 const int u = i * kGroups + gi, v = i * (kGroups - 1) + gi;
-                const uint32_t pair = lds32(scale_at + (i % kWideXBuffers) * Shape::kScaleBytes + (gi * kLoaders + lt) * 4);
-                const float2 both = scale_pair(pair, p.scale_bf16);
+                const float2 both = scale_pair(scales[gi], p.scale_bf16);
                 const float sc = lane & 8 ? both.y : both.x;
                 ok = ok && (gi == kGroups - 1 ? wait(&done[i % kAB], i / kAB) : wait(&part_done[v & 1], v >> 1));
                 if (!ok) break;
@@ -427,13 +469,15 @@ w4_wide_kernel(const LinearParams p) {
                     }
                 }
             }
+            if (!ok) break;
+            publish(i + 2);  // D of chunk i is in registers
+#pragma unroll
+            for (int gi = 0; gi < kGroups; ++gi) scales[gi] = scales1[gi], scales1[gi] = scales2[gi];
         }
-        cp_async_wait<0>();
-        // The last group's D is complete, so no MMA reads X and no warp converts
-        // any more, and behind this barrier no warp reads a scale: the partial
-        // sums go over them.
-        asm volatile("bar.sync 1, %0;" ::"n"(kLoaders) : "memory");
-        float* part = reinterpret_cast<float*>(smem) + set * Shape::kCols * kWidePartStride + quarter * 32 + lane;
+        // The last chunk is multiplied, so no MMA reads X and no warp converts any
+        // more: the partial sums go over them.
+        if (kTurns > 1 && n > 0 && ok) ok = wait(&done[(n - 1) % kAB], (n - 1) / kAB);
+        float* part = reinterpret_cast<float*>(smem) + (turn * NT + set * Shape::kCols) * kWidePartStride + quarter * 32 + lane;
         const float poison = ok && !s_failed ? 0.0f : __int_as_float(0x7fffffff);
 #pragma unroll
         for (int e = 0; e < Shape::kCols; ++e) part[e * kWidePartStride] = acc[e] + poison;
@@ -445,22 +489,46 @@ w4_wide_kernel(const LinearParams p) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Shape::kTmemCols));
     }
     if (p.cluster > 1) cluster_barrier();
-    const int64_t row0 = block * kWideRows;
-    for (int e = rank * Shape::kThreads + threadIdx.x; e < tokens * kWideRows; e += Shape::kThreads * p.cluster) {
-        const int token = e / kWideRows, row = e % kWideRows;
-        if (row0 + row >= p.n) continue;
-        const uint32_t at = xs + (token * kWidePartStride + row) * 4;
-        float v = 0.0f;
-        if (p.cluster > 1)
-            for (int c = 0; c < p.cluster; ++c) v += ld_cluster(at, c);
-        else
-            v = __uint_as_float(lds32(at));
-        const int64_t out_row = token0 + token;
-        v *= ZEROS && KIND == kI8 ? 1.0f : A::kScale;
-        if (p.x_scale) v *= p.x_scale[out_row];
-        if (p.bias) v += load_as_float(p.bias, row0 + row, p.out_dtype);
-        if (p.residual) v += load_as_float(p.residual, out_row * p.residual_stride + row0 + row, p.out_dtype);
-        store_from_float(p.out, out_row * p.out_stride + row0 + row, p.out_dtype, v);
+    // A thread keeps to one row and has eight tokens' residuals under way, as raw
+    // bits: one at a time, their latencies were a third of a call.
+    constexpr int kLines = Shape::kThreads / kWideRows, kPer = 8;
+    const int row = threadIdx.x % kWideRows;
+    const int64_t column = block * kWideRows + row;
+    if (threadIdx.x < kLines * kWideRows && column < p.n) {
+        const int step = kLines * p.cluster;
+        const bool wide = p.out_dtype == kF32;
+        for (int t0 = rank * kLines + threadIdx.x / kWideRows; t0 < tokens; t0 += kPer * step) {
+            uint32_t bits[kPer] = {};
+            if (p.residual) {
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) {
+                    const int64_t at = (token0 + t0 + j * step) * p.residual_stride + column;
+                    if (t0 + j * step < tokens)
+                        bits[j] = wide ? static_cast<const uint32_t*>(p.residual)[at] : static_cast<const uint16_t*>(p.residual)[at];
+                }
+            }
+#pragma unroll 1
+            for (int j = 0; j < kPer; ++j) {
+                const int token = t0 + j * step;
+                if (token >= tokens) break;
+                const uint32_t at = xs + (token * kWidePartStride + row) * 4;
+                float v = 0.0f;
+                for (int c = 0; c < p.cluster; ++c)
+#pragma unroll
+                    for (int turn = 0; turn < kTurns; ++turn) {
+                        const uint32_t from = at + turn * NT * kWidePartStride * 4;
+                        v += p.cluster > 1 ? ld_cluster(from, c) : __uint_as_float(lds32(from));
+                    }
+                uint32_t b = bits[0];
+#pragma unroll
+                for (int i = 0; i + 1 < kPer; ++i) bits[i] = bits[i + 1];
+                const float residual = wide ? __uint_as_float(b)
+                                       : p.out_dtype == kBF16 ? __uint_as_float(b << 16)
+                                                              : __half2float(__ushort_as_half(static_cast<uint16_t>(b)));
+                store_from_float(p.out, (token0 + token) * p.out_stride + column, p.out_dtype,
+                                 fmaf(v, s_scale[token], s_bias[row]) + residual);
+            }
+        }
     }
     if (p.cluster > 1) cluster_barrier();  // no CTA leaves while another reads its shared memory
 }
