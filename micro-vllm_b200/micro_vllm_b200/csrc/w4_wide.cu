@@ -42,20 +42,26 @@ int x_map(const LinearParams& p, int kind, int rows, CUtensorMap* map) {
     return MVQ_OK;
 }
 
-// CTAs that share a block of rows' columns: the number in 1..8 with the least
-// estimated time. An SM takes its share of the CTAs; each costs `start` and its
-// chunks. WIDE_NOTE
+// CTAs that share a block of rows' columns, with the least estimated time (us).
+// Fitted to calls of 896 x 1152 to 8192 x 57344: a call starts and ends in about
+// five (with 64 tokens and one CTA per SM, ten); a chunk takes 0.33 us of a CTA
+// alone on its SM, 0.22 of an SM with two, and up to 0.53 with 128 tokens; a
+// cluster costs its barriers. Measured on both sides: 3584 x 28672 at 16 rows 22.7
+// us alone, 27.7 in pairs; 14336 x 3584 at 64 rows 52.0 alone, 20.2 in fours, 30.7
+// in eights (two rounds). Clusters of five and seven do not fill the SMs' groups.
 int wide_cluster(int64_t blocks, int chunks, int sms, int nt) {
 #ifdef MVQ_TUNE
     if (getenv("CL")) return atoi(getenv("CL"));
 #endif
-    const double start = nt <= 32 ? 4.0 : nt == 64 ? 6.5 : 9.0;
-    const double chunk = nt == 16 ? 0.3 : nt == 32 ? 0.33 : nt == 64 ? 0.59 : 0.75;
     int best = 1;
     double least = 0.0;
-    for (int c = 1; c <= 8 && c <= chunks; ++c) {
+    for (int c : {1, 2, 3, 4, 6, 8}) {
+        if (c > chunks) break;
         const int64_t per_sm = (blocks * c + sms - 1) / sms;
-        const double time = static_cast<double>(per_sm) * (start + chunk * ((chunks + c - 1) / c));
+        const int run = (chunks + c - 1) / c;
+        double time = c > 1 ? 0.3 * c : 0.0;
+        if (nt >= 64) time += per_sm * (9.7 + run * (nt == 64 ? 0.38 : 0.53));
+        else time += 5.2 + (per_sm <= 1 ? run * 0.33 : per_sm * (3.0 + run * 0.22));
         if (c == 1 || time < least) least = time, best = c;
     }
     return best;

@@ -170,8 +170,9 @@ w4_wide_kernel(const LinearParams p, const __grid_constant__ CUtensorMap xmap) {
     extern __shared__ uint8_t smem_raw[];
     // full: a chunk's A and X are in place and D of the chunk two before is
     // drained. done: its last group is multiplied, which frees A and X and hands
-    // over D. part_done and d_empty only serve chunks of several groups.
-    __shared__ __align__(8) uint64_t full[kAB], done[kAB], part_done[2], d_empty[2], drained;
+    // over D. part_done and d_empty only serve chunks of several groups; each turn
+    // has its own part_done, since a waiter may not skip a phase of a barrier.
+    __shared__ __align__(8) uint64_t full[kAB], done[kAB], part_done[kTurns][2], d_empty[2], drained;
     __shared__ uint32_t s_tmem;
     __shared__ float s_scale[NT], s_bias[kWideRows];
     __shared__ volatile int s_failed;
@@ -205,7 +206,7 @@ w4_wide_kernel(const LinearParams p, const __grid_constant__ CUtensorMap xmap) {
             mv::mbar_init(mv::smem_addr(&done[i]), 1);
         }
         for (int i = 0; i < 2; ++i) {
-            mv::mbar_init(mv::smem_addr(&part_done[i]), 1);
+            for (int turn = 0; turn < kTurns; ++turn) mv::mbar_init(mv::smem_addr(&part_done[turn][i]), 1);
             mv::mbar_init(mv::smem_addr(&d_empty[i]), 4 * kSets);
         }
         mv::mbar_init(mv::smem_addr(&drained), 1);
@@ -341,8 +342,8 @@ w4_wide_kernel(const LinearParams p, const __grid_constant__ CUtensorMap xmap) {
                     const uint32_t b = KIND == kI8 ? x_at + step * 32 : x_at + (step >> 2) * (NT * 128) + (step & 3) * 32;
                     wide_mma<KIND>(leader, d_col + (u & 1) * NT, a_at + s * 8, sw128_desc(b), wide_idesc<KIND, NT>(), s > 0);
                 }
-                wide_commit(leader, mv::smem_addr(gi == kGroups - 1 ? &done[i % kAB]
-                                                                    : &part_done[(i * (kGroups - 1) + gi) & 1]));
+                const int v = i / kTurns * (kGroups - 1) + gi;
+                wide_commit(leader, mv::smem_addr(gi == kGroups - 1 ? &done[i % kAB] : &part_done[i % kTurns][v & 1]));
             }
             if (!ok) break;
         }
@@ -443,10 +444,10 @@ w4_wide_kernel(const LinearParams p, const __grid_constant__ CUtensorMap xmap) {
                                                              lane * 128));
 #pragma unroll
             for (int gi = 0; gi < kGroups; ++gi) {
-                const int u = i * kGroups + gi, v = i * (kGroups - 1) + gi;
+                const int u = i * kGroups + gi, v = i / kTurns * (kGroups - 1) + gi;
                 const float2 both = scale_pair(scales[gi], p.scale_bf16);
                 const float sc = lane & 8 ? both.y : both.x;
-                ok = ok && (gi == kGroups - 1 ? wait(&done[i % kAB], i / kAB) : wait(&part_done[v & 1], v >> 1));
+                ok = ok && (gi == kGroups - 1 ? wait(&done[i % kAB], i / kAB) : wait(&part_done[turn][v & 1], v >> 1));
                 if (!ok) break;
                 fence_after();
                 const uint32_t from = lanes + (u & 1) * NT;

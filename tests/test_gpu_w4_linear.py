@@ -78,6 +78,35 @@ def test_token_counts(dtype, m):
 
 
 @pytest.mark.parametrize('dtype', FLOATS + [torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize('group', [32, 64, 128])
+@pytest.mark.parametrize('zeros', [False, True])
+@pytest.mark.parametrize('m', [12, 30, 33, 64, 65, 128, 130])
+@pytest.mark.parametrize('k', [840, 1153])
+def test_groups_at_every_token_block(dtype, group, zeros, m, k):
+    from micro_vllm_b200.w4_linear import w4_linear
+    weight, w = make(200, k, group, zeros, seed=m + k)
+    x, scale = activations(m, k, dtype, seed=k)
+    out_dtype = dtype if dtype in FLOATS else torch.bfloat16
+    y = w4_linear(x.cuda(), weight, x_scale=None if scale is None else scale.cuda(), out_dtype=out_dtype)
+    assert_linear(y, x, scale, w, group=group)
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.int8])
+@pytest.mark.parametrize('group', [32, 64, 128])
+@pytest.mark.parametrize('m', [16, 64, 128])
+def test_long_columns_of_every_group_and_token_block(dtype, group, m):
+    """Many turns of every buffer and barrier, with bias and residual."""
+    from micro_vllm_b200.w4_linear import w4_linear
+    k, n = 14336, 384
+    gen = torch.Generator().manual_seed(m)
+    weight, w = make(n, k, group, True, seed=m)
+    x, scale = activations(m, k, dtype, seed=group)
+    bias, residual = torch.randn(n, generator=gen).bfloat16(), torch.randn((m, n), generator=gen).bfloat16()
+    y = w4_linear(x.cuda(), weight, bias.cuda(), residual.cuda(), x_scale=None if scale is None else scale.cuda())
+    assert_linear(y, x, scale, w, bias, residual, group=group)
+
+
+@pytest.mark.parametrize('dtype', FLOATS + [torch.int8, torch.float8_e4m3fn])
 @pytest.mark.parametrize('k', [1, 2, 7, 8, 31, 33, 127, 129, 255, 1001, 4097])
 @pytest.mark.parametrize('n', [1, 63, 65])
 def test_odd_sizes(dtype, k, n):
