@@ -4,8 +4,13 @@ Every entry point takes one struct of 8-byte fields and a stream. The struct is
 packed into an immutable bytes object for each call (one C call instead of a
 marshalled argument each), so calls from several threads share nothing. As with
 libmvdecode.so the library is loaded on first use and there is no fallback.
+
+``binding()`` is the same entry points' usual calls as Python functions
+(csrc/mvq_binding.cpp), which return None for every call that is not usual.
 """
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import struct
 from functools import lru_cache
@@ -15,6 +20,8 @@ from . import _native
 
 # MVQUANT_LIBRARY may name another build of the same library (e.g. a tuning variant).
 LIB_PATH = Path(os.environ.get('MVQUANT_LIBRARY', Path(__file__).resolve().parent / 'lib' / 'libmvquant.so'))
+
+BINDING_PATH = Path(__file__).resolve().parent / 'lib' / '_mvq_binding.so'
 
 MVQ_ABI_VERSION = 1
 DTYPE_F32, DTYPE_F16, DTYPE_BF16, DTYPE_I8, DTYPE_E4M3 = 0, 1, 2, 3, 4
@@ -26,6 +33,10 @@ DEQUANTIZE_FIELDS = ('records', 'n', 'k', 'group', 'has_zeros', 'scale_dtype', '
 NORM_FIELDS = ('x', 'x_stride_row', 'residual', 'residual_stride_row', 'weight', 'out', 'out_stride_row', 'scales',
                'residual_out', 'residual_out_stride_row', 'rows', 'hidden', 'eps', 'dtype', 'out_dtype')
 SILU_FIELDS = ('gate_up', 'stride_row', 'out', 'out_stride_row', 'scales', 'rows', 'width', 'dtype', 'out_dtype')
+
+
+# The fields that describe a weight, the same in two structs.
+pack_weight = struct.Struct('=6q').pack
 
 
 def _packer(fields):
@@ -64,6 +75,21 @@ def library() -> ctypes.CDLL:
     if version != MVQ_ABI_VERSION:
         raise RuntimeError(f'libmvquant ABI {version}, expected {MVQ_ABI_VERSION}')
     return lib
+
+
+@lru_cache(maxsize=1)
+def binding():
+    """Load _mvq_binding.so once and give it the library's entry points."""
+    if not BINDING_PATH.exists():
+        raise RuntimeError(
+            f'{BINDING_PATH} is not built: run `python -m micro_vllm_b200.build` '
+            '(or __graft_entry__.build()) before using the CUDA kernels')
+    lib = library()
+    loader = importlib.machinery.ExtensionFileLoader('_mvq_binding', str(BINDING_PATH))
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader('_mvq_binding', loader))
+    loader.exec_module(module)
+    module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in ENTRY_POINTS))
+    return module
 
 
 def check(status: int) -> None:

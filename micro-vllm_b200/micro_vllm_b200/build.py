@@ -1,9 +1,11 @@
-"""Build libmvdecode.so and libmvquant.so in-tree for sm_100a with nvcc.
+"""Build libmvdecode.so, libmvquant.so and its Python binding in-tree for sm_100a.
 
     python -m micro_vllm_b200.build        (from the micro-vllm_b200/ source root)
 
 libmvdecode.so holds the decode path (include/mvdecode.h), libmvquant.so the
-operators with 4-bit weights and 8-bit rows (include/mvquant.h). Both link the
+operators with 4-bit weights and 8-bit rows (include/mvquant.h), _mvq_binding.so
+their common calls as Python functions (torch's C++ API, host code only). Both
+libraries link the
 CUDA runtime statically and the first resolves the driver's tensor-map encoder
 at run time, so they need only the NVIDIA driver next to them.
 """
@@ -12,6 +14,7 @@ import re
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PACKAGE_DIR = Path(__file__).resolve().parent
@@ -19,6 +22,7 @@ CSRC_DIR = PACKAGE_DIR / 'csrc'
 LIB_DIR = PACKAGE_DIR / 'lib'
 LIB_PATH = LIB_DIR / 'libmvdecode.so'
 QUANT_LIB_PATH = LIB_DIR / 'libmvquant.so'
+BINDING_PATH = LIB_DIR / '_mvq_binding.so'
 INCLUDE_DIR = PACKAGE_DIR.parents[1] / 'include'
 
 NVCC_FLAGS = [
@@ -46,7 +50,27 @@ LIBRARIES = {
     LIB_PATH: ([CSRC_DIR / 'mv_capi.cu'], INCLUDE_DIR / 'mvdecode.h'),
     QUANT_LIB_PATH: ([CSRC_DIR / 'mvq_capi.cu', CSRC_DIR / 'w4_linear.cu', CSRC_DIR / 'w4_wide.cu'],
                      INCLUDE_DIR / 'mvquant.h'),
+    BINDING_PATH: ([CSRC_DIR / 'mvq_binding.cpp'], INCLUDE_DIR / 'mvquant.h'),
 }
+
+
+def _command(library: Path, tmp: Path, units, verbose: bool):
+    """The compiler call that makes a library of its units."""
+    if library != BINDING_PATH:
+        cmd = [nvcc_path(), *NVCC_FLAGS, '-I', str(INCLUDE_DIR), '--threads', str(len(units)),
+               '-o', str(tmp), *map(str, units)]
+        if verbose:
+            cmd.insert(1, '-Xptxas=-v')
+        return cmd
+    import torch
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc_path()).resolve().parents[1]
+    includes = [root / 'include', root / 'include/torch/csrc/api/include', cuda / 'include',
+                sysconfig.get_paths()['include'], INCLUDE_DIR]
+    return [os.environ.get('CXX', 'g++'), '-O2', '-std=c++17', '-shared', '-fPIC', '-fvisibility=hidden',
+            f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}', *(f'-I{path}' for path in includes),
+            '-o', str(tmp), *map(str, units), f'-L{root / "lib"}', '-lc10', '-lc10_cuda', '-ltorch_cpu', '-ltorch_cuda',
+            '-ltorch_python']
 
 
 def _reached(path: Path, seen=None):
@@ -81,10 +105,8 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         if not force and not _library_is_stale(library):
             continue
         tmp = library.with_suffix('.so.tmp')
-        cmd = [nvcc_path(), *NVCC_FLAGS, '-I', str(INCLUDE_DIR), '--threads', str(len(units)),
-               '-o', str(tmp), *map(str, units)]
+        cmd = _command(library, tmp, units, verbose)
         if verbose:
-            cmd.insert(1, '-Xptxas=-v')
             print(' '.join(cmd), file=sys.stderr)
         running.append((library, tmp, cmd, subprocess.Popen(cmd)))
     codes = [process.wait() for *_, process in running]

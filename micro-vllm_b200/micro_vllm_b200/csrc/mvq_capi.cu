@@ -202,9 +202,15 @@ int mvq_w4_linear(const MvqLinearArgs* a, void* stream) try {
                                a->x_stride_row < (int64_t(1) << 38)));
     const int kind = a->x_dtype == MVQ_DTYPE_E4M3 ? mvq::kF16 : static_cast<int>(a->x_dtype);
     const int group = static_cast<int>(a->group);
-    int few = 8;
+    // The mma.sync kernel up to eight rows, except for five to eight rows of small
+    // weights, where staging x and joining sums outweigh the stream (measured at eight:
+    // 896 x 1152 3.6 to 4.0 us wide, 6.0 narrow; 14336 x 3584 in bf16 15.1 and 17.3, in
+    // int8 14.7 and 13.4; 3584 x 28672 in bf16 21.4 both, in int8 18.0 and 15.6).
+    const bool small = p.chunks <= 16 || (kind != mvq::kI8 && p.tiles <= 64);
 #ifdef MVQ_TUNE
-    if (getenv("FEW")) few = atoi(getenv("FEW"));
+    const int few = getenv("FEW") ? atoi(getenv("FEW")) : small ? 4 : 8;
+#else
+    const int few = small ? 4 : 8;
 #endif
     if (kind == mvq::kF32 || a->m <= few)
         return mvq::launch_narrow(p, kind, group, a->has_zeros != 0, device, sms, stream);

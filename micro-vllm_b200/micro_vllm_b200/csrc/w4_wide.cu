@@ -42,28 +42,32 @@ int x_map(const LinearParams& p, int kind, int rows, CUtensorMap* map) {
     return MVQ_OK;
 }
 
-// CTAs that share a block of rows' columns, with the least estimated time (us).
-// Fitted to calls of 896 x 1152 to 8192 x 57344: a call starts and ends in about
-// five (with 64 tokens and one CTA per SM, ten); a chunk takes 0.33 us of a CTA
-// alone on its SM, 0.22 of an SM with two, and up to 0.53 with 128 tokens; a
-// cluster costs its barriers. Measured on both sides: 3584 x 28672 at 16 rows 22.7
-// us alone, 27.7 in pairs; 14336 x 3584 at 64 rows 52.0 alone, 20.2 in fours, 30.7
-// in eights (two rounds). Clusters of five and seven do not fill the SMs' groups.
-int wide_cluster(int64_t blocks, int chunks, int sms, int nt) {
+constexpr int kClusters[] = {1, 2, 3, 4, 6, 8};
+
+// CTAs that share a block of rows' columns: the kClusters number with the least
+// estimated time (us); slots[i]: how many clusters of kClusters[i] the device holds
+// at once. Fitted to calls of 896 x 1152 to 8192 x 57344: a call starts and ends in
+// about five (with 64 tokens and one CTA per SM, ten); a chunk takes 0.33 us of a
+// CTA alone on its SM, 0.22 of an SM with two, and up to 0.53 with 128 tokens; a
+// cluster costs its barriers. Both sides measured: 3584 x 28672 at 16 rows 22.7 us
+// alone, 27.7 in pairs; 14336 x 3584 at 64 rows 52.0 alone, 20.2 in fours, 30.7 in
+// eights, of which not all fit at once.
+int wide_cluster(int64_t blocks, int chunks, int nt, const int* slots) {
+    int best = 1;
+    double least = 0.0;
+    for (int i = 0; i < 6; ++i) {
+        const int c = kClusters[i];
+        if (c > chunks || slots[i] <= 0) break;
+        const double rounds = static_cast<double>((blocks + slots[i] - 1) / slots[i]);
+        const int run = (chunks + c - 1) / c;
+        double time = c > 1 ? 0.3 * c : 0.0;
+        if (nt >= 64) time += rounds * (9.7 + run * (nt == 64 ? 0.38 : 0.53));
+        else time += 5.2 + (2 * blocks <= slots[i] ? run * 0.33 : 2 * rounds * (3.0 + run * 0.22));
+        if (c == 1 || time < least) least = time, best = c;
+    }
 #ifdef MVQ_TUNE
     if (getenv("CL")) return atoi(getenv("CL"));
 #endif
-    int best = 1;
-    double least = 0.0;
-    for (int c : {1, 2, 3, 4, 6, 8}) {
-        if (c > chunks) break;
-        const int64_t per_sm = (blocks * c + sms - 1) / sms;
-        const int run = (chunks + c - 1) / c;
-        double time = c > 1 ? 0.3 * c : 0.0;
-        if (nt >= 64) time += per_sm * (9.7 + run * (nt == 64 ? 0.38 : 0.53));
-        else time += 5.2 + (per_sm <= 1 ? run * 0.33 : per_sm * (3.0 + run * 0.22));
-        if (c == 1 || time < least) least = time, best = c;
-    }
     return best;
 }
 
@@ -75,6 +79,7 @@ int launch_one(LinearParams p, int device, int sms, void* stream) {
     static_assert(kSmem <= kSmemMost, "shared memory");
     static std::mutex mutex;
     static bool ready[kMaxDevices];
+    static int slots[kMaxDevices][6];  // clusters of each kClusters size that the device holds at once
     {
         std::lock_guard<std::mutex> lock(mutex);
         if (!ready[device]) {
@@ -83,13 +88,27 @@ int launch_one(LinearParams p, int device, int sms, void* stream) {
                 err = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
                                            static_cast<int>(cudaSharedmemCarveoutMaxShared));
             if (err != cudaSuccess) return cuda_fail(err, "cudaFuncSetAttribute");
+            for (int i = 0; i < 6; ++i) {
+                cudaLaunchConfig_t cfg = {};
+                cfg.gridDim = dim3(kClusters[i] * sms);
+                cfg.blockDim = dim3(Shape::kThreads);
+                cfg.dynamicSmemBytes = kSmem;
+                cudaLaunchAttribute attr;
+                attr.id = cudaLaunchAttributeClusterDimension;
+                attr.val.clusterDim.x = kClusters[i];
+                attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+                cfg.attrs = &attr;
+                cfg.numAttrs = 1;
+                err = cudaOccupancyMaxActiveClusters(&slots[device][i], kernel, &cfg);
+                if (err != cudaSuccess) return cuda_fail(err, "cudaOccupancyMaxActiveClusters");
+            }
             ready[device] = true;
         }
     }
     const int64_t blocks = (static_cast<int64_t>(p.n) + kWideRows - 1) / kWideRows;
     const int64_t passes = (static_cast<int64_t>(p.m) + NT - 1) / NT;
     if (passes > 65535) return fail(MVQ_ERR_UNSUPPORTED, "too many rows of x for one call");
-    p.cluster = wide_cluster(blocks * passes, p.chunks, sms, NT);
+    p.cluster = wide_cluster(blocks * passes, p.chunks, NT, slots[device]);
     CUtensorMap map = {};
     if (p.x_units) {
         const int rc = x_map(p, KIND, NT, &map);

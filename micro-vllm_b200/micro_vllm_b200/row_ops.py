@@ -125,6 +125,11 @@ def _launch(entry, packed, index):
 
 
 def _add_rms_norm(x, residual, weight, eps, out, out_dtype, scales, residual_out):
+    if out is None and scales is None and residual_out is None and x.is_cuda:
+        found = _quant_native.binding().norm(x, residual, weight, eps, out_dtype)
+        if found is not None:
+            return found
+    # Not the usual call: everything is checked, and refused with its reason, here.
     dtype, shape = x.dtype, x.shape
     code = DTYPE_CODES.get(dtype)
     _check(x.is_cuda and code is not None and shape, 'row operations take CUDA float tensors')
@@ -208,6 +213,10 @@ def silu_mul_quant(gate_up: torch.Tensor, *, quant_dtype: torch.dtype = torch.in
     """
     out_code = QUANT_CODES.get(quant_dtype)
     _check(out_code is not None, 'quant_dtype must be int8 or float8_e4m3fn')
+    if out is None and scales is None and gate_up.is_cuda:
+        found = _quant_native.binding().silu(gate_up, quant_dtype)
+        if found is not None:
+            return found
     dtype, shape = gate_up.dtype, gate_up.shape
     code = DTYPE_CODES.get(dtype)
     _check(gate_up.is_cuda and code is not None and shape, 'row operations take CUDA float tensors')

@@ -39,7 +39,7 @@ def _check(condition, message):
 class W4Weight:
     """A [N, K] weight in 4-bit codes, laid out for the kernels (include/mvquant.h). Immutable."""
 
-    __slots__ = ('records', 'shape', 'group_size', 'has_zeros', 'scale_dtype', 'index', 'fixed')
+    __slots__ = ('records', 'shape', 'group_size', 'has_zeros', 'scale_dtype', 'index', 'fixed', 'packed')
 
     def __init__(self, records, shape, group_size, has_zeros, scale_dtype):
         self.records = records
@@ -50,6 +50,7 @@ class W4Weight:
         self.index = records.get_device()  # -1 on the CPU
         # The weight's fields of the calls' argument structs.
         self.fixed = (records.data_ptr(), *self.shape, group_size, int(has_zeros), SCALE_CODES[scale_dtype])
+        self.packed = _native.pack_weight(*self.fixed)
 
     @property
     def device(self):
@@ -196,6 +197,11 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, bias: torch.Tensor | None = Non
     of these. bias [N] and residual [..., N] have that type; out may be residual.
     Any number of rows; made for a decode step's (up to 128). Runs on the current stream.
     """
+    if out is None and x.is_cuda:
+        y = _native.binding().linear(x, weight.packed, weight.index, bias, residual, x_scale, out_dtype)
+        if y is not None:
+            return y
+    # Not the usual call: everything is checked, and refused with its reason, here.
     n, k = weight.shape
     x_dtype = x.dtype
     code = ACTIVATION_CODES.get(x_dtype)
@@ -274,6 +280,10 @@ def w4_dequantize(weight: W4Weight, dtype: torch.dtype | None = None, *,
     index = weight.index
     _check(index >= 0, 'the weight must be on a CUDA device')
     dtype = dtype or (out.dtype if out is not None else weight.scale_dtype)
+    if out is None:
+        out = _native.binding().dequantize(weight.packed, weight.records, dtype)
+        if out is not None:
+            return out
     code = FLOAT_CODES.get(dtype)
     _check(code is not None, 'dtype must be float32, float16 or bfloat16')
     if out is None:
