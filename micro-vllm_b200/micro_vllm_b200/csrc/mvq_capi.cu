@@ -230,10 +230,11 @@ int mvq_w4_dequantize(const MvqDequantizeArgs* a, void* stream) try {
         return fail(MVQ_ERR_INVALID_ARGUMENT, "out's rows must not overlap");
     const int chunks = static_cast<int>((a->k + mvq::kChunk - 1) / mvq::kChunk);
     const int64_t total = (a->n + mvq::kTileRows - 1) / mvq::kTileRows * chunks;
-    if (total >= (int64_t(1) << 33)) return fail(MVQ_ERR_UNSUPPORTED, "the weight is too large for one call");
+    if (total >= (int64_t(1) << 31)) return fail(MVQ_ERR_UNSUPPORTED, "the weight is too large for one call");
     const int64_t size = dtype_size(a->out_dtype);
     const int runs = address(a->out) % 16 == 0 && (a->n == 1 || a->out_stride_row * size % 16 == 0);
-    const dim3 grid(static_cast<unsigned>((total + 7) / 8));
+    // A warp per 32 columns of a record.
+    const dim3 grid(static_cast<unsigned>((4 * total + mvq::kDequantizeWarps - 1) / mvq::kDequantizeWarps));
     const int bytes = mvq::record_size(static_cast<int>(a->group), a->has_zeros != 0), bf16 = a->scale_dtype == MVQ_DTYPE_BF16;
     const uint8_t* records = static_cast<const uint8_t*>(a->records);
     const int group = static_cast<int>(a->group), zeros = a->has_zeros != 0;

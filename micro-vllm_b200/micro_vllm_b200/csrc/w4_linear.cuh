@@ -595,7 +595,10 @@ __global__ void __launch_bounds__(kThreads, 4) w4_linear_kernel(const LinearPara
     if (p.cluster > 1) cluster_barrier();  // no CTA leaves while another reads its shared memory
 }
 
-// W written out, rounded once: a warp per record. Bound by the output's bytes.
+// W written out, rounded once: a warp per 32 columns of a record, the smallest
+// piece that holds whole words (a record each took a small weight 5.9 us instead of
+// 2.3 for 896 x 1152, for one warp's chain of steps, and 3584 x 28672 45.0 instead of
+// 40.5). Bound by the output's bytes.
 // A code's distance from its zero point is exact in 16 bits, and its product
 // with a scale has at most 4 + 11 bits, so that a 16-bit product with a scale of
 // the output's type (`same`) rounds exactly as the fp32 product does.
@@ -625,7 +628,9 @@ w4_dequantize_kernel(const uint8_t* records, int64_t total, int chunks, int reco
     constexpr bool kBf16 = std::is_same<Kind, Act<kBF16>>::value;
     mv::wait_for_prior_grid();
     mv::allow_next_grid();
-    const int64_t id = static_cast<int64_t>(blockIdx.x) * kDequantizeWarps + (threadIdx.x >> 5);
+    const int64_t piece = static_cast<int64_t>(blockIdx.x) * kDequantizeWarps + (threadIdx.x >> 5);
+    const int64_t id = piece >> 2;
+    const int h = static_cast<int>(piece & 3);
     if (id >= total) return;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int64_t tile = id / chunks;
@@ -636,24 +641,25 @@ w4_dequantize_kernel(const uint8_t* records, int64_t total, int chunks, int reco
     // Rows that are not aligned go out through shared memory, so that a warp
     // stores 32 columns of one row at a time.
     __shared__ T rows_out[sizeof(T) == 2 ? kDequantizeWarps : 1][sizeof(T) == 2 ? 64 * 34 : 1];
-    uint4 codes[4][2];
+    uint4 codes[2];
 #pragma unroll
-    for (int h = 0; h < 4; ++h)
-#pragma unroll
-        for (int rp = 0; rp < 2; ++rp) codes[h][rp] = __ldg(reinterpret_cast<const uint4*>(rec) + (h * 2 + rp) * 32 + lane);
-#pragma unroll
-    for (int h = 0; h < 4; ++h) {
+    for (int rp = 0; rp < 2; ++rp) codes[rp] = __ldg(reinterpret_cast<const uint4*>(rec) + (h * 2 + rp) * 32 + lane);
+    {
         const int gi = h / group_runs;
-        // Two lanes trade words, so that each holds eight columns in a row: the
-        // even one both quads of the first half of h, the odd one of the second.
-        const int c0 = k0 + 32 * h + 16 * (t & 1) + 4 * (t & 2);
+        // 16 bits: two lanes trade words, so that each holds eight columns in a row,
+        // 16 bytes: the even one both quads of the first half of h, the odd one of the
+        // second. fp32: a quad is 16 bytes as it is.
+        constexpr bool kTrade = sizeof(T) == 2;
+        const int c0 = k0 + 32 * h + (kTrade ? 16 * (t & 1) + 4 * (t & 2) : 4 * t);
 #pragma unroll
         for (int rp = 0; rp < 2; ++rp) {
-            uint4 w = codes[h][rp];
-            const uint32_t got0 = __shfl_xor_sync(0xffffffffu, t & 1 ? w.x : w.y, 1);
-            const uint32_t got1 = __shfl_xor_sync(0xffffffffu, t & 1 ? w.z : w.w, 1);
-            if (t & 1) w.x = got0, w.z = got1;
-            else w.y = got0, w.w = got1;
+            uint4 w = codes[rp];
+            if constexpr (kTrade) {
+                const uint32_t got0 = __shfl_xor_sync(0xffffffffu, t & 1 ? w.x : w.y, 1);
+                const uint32_t got1 = __shfl_xor_sync(0xffffffffu, t & 1 ? w.z : w.w, 1);
+                if (t & 1) w.x = got0, w.z = got1;
+                else w.y = got0, w.w = got1;
+            }
             const uint2 s = __ldg(reinterpret_cast<const uint2*>(rec + kCodeBytes + gi * 128 + g * 16 + rp * 8));
             uint32_t z = 0;
             if (has_zeros) z = __ldg(reinterpret_cast<const uint32_t*>(rec + kCodeBytes + groups * 128 + gi * 64 + g * 8 + rp * 4));
@@ -697,26 +703,29 @@ w4_dequantize_kernel(const uint8_t* records, int64_t total, int chunks, int reco
                         }
                     }
                     T* dst = out + row * out_stride + c0;
-                    if (runs && c0 + 8 <= k) {
-                        if constexpr (sizeof(T) == 2) {
-                            *reinterpret_cast<uint4*>(dst) = make_uint4(v[0], v[1], v[2], v[3]);
-                        } else {
-                            reinterpret_cast<float4*>(dst)[0] = make_float4(f[0], f[1], f[2], f[3]);
-                            reinterpret_cast<float4*>(dst)[1] = make_float4(f[4], f[5], f[6], f[7]);
-                        }
-                    } else if (runs || sizeof(T) == 4) {
+                    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            if (row < n && c0 + i < k) {
-                                if constexpr (sizeof(T) == 2) {
-                                    const uint16_t bits = static_cast<uint16_t>(v[i >> 1] >> (16 * (i & 1)));
-                                    dst[i] = *reinterpret_cast<const T*>(&bits);
-                                } else {
-                                    dst[i] = f[i];
-                                }
+                        for (int quad = 0; quad < 2; ++quad) {
+                            const int c = c0 + 16 * quad;
+                            if (row >= n) break;
+                            if (runs && c + 4 <= k) {
+                                *reinterpret_cast<float4*>(dst + 16 * quad) =
+                                    make_float4(f[4 * quad], f[4 * quad + 1], f[4 * quad + 2], f[4 * quad + 3]);
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    if (c + i < k) dst[16 * quad + i] = f[4 * quad + i];
                             }
                         }
-                    } else if constexpr (sizeof(T) == 2) {
+                    } else if (runs && c0 + 8 <= k) {
+                        *reinterpret_cast<uint4*>(dst) = make_uint4(v[0], v[1], v[2], v[3]);
+                    } else if (runs) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const uint16_t bits = static_cast<uint16_t>(v[i >> 1] >> (16 * (i & 1)));
+                            if (c0 + i < k) dst[i] = *reinterpret_cast<const T*>(&bits);
+                        }
+                    } else {
                         uint32_t* at = reinterpret_cast<uint32_t*>(
                             &rows_out[threadIdx.x >> 5][(32 * rp + 16 * q + 8 * half + g) * 34 + 16 * (t & 1) + 4 * (t & 2)]);
 #pragma unroll
