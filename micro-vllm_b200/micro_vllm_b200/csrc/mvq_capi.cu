@@ -2,7 +2,6 @@
 #include "mvquant.h"
 
 #include <cmath>
-#include <cstdlib>
 #include <cstdarg>
 #include <cstdio>
 #include <mutex>
@@ -207,11 +206,7 @@ int mvq_w4_linear(const MvqLinearArgs* a, void* stream) try {
     // 896 x 1152 3.6 to 4.0 us wide, 6.0 narrow; 14336 x 3584 in bf16 15.1 and 17.3, in
     // int8 14.7 and 13.4; 3584 x 28672 in bf16 21.4 both, in int8 18.0 and 15.6).
     const bool small = p.chunks <= 16 || (kind != mvq::kI8 && p.tiles <= 64);
-#ifdef MVQ_TUNE
-    const int few = getenv("FEW") ? atoi(getenv("FEW")) : small ? 4 : 8;
-#else
     const int few = small ? 4 : 8;
-#endif
     if (kind == mvq::kF32 || a->m <= few)
         return mvq::launch_narrow(p, kind, group, a->has_zeros != 0, device, sms, stream);
     return mvq::launch_wide(p, kind, group, a->has_zeros != 0, device, sms, stream);

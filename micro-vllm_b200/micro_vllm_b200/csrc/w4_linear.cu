@@ -1,6 +1,5 @@
 // Plans and launches of the mma.sync product kernel (w4_linear.cuh).
 #include <algorithm>
-#include <cstdlib>
 #include <mutex>
 
 #include "mvq_host.cuh"
@@ -47,11 +46,6 @@ LinearPlan linear_plan(int64_t m, int64_t chunks, int64_t tiles, int kind, int r
             }
         }
     }
-#ifdef MVQ_TUNE
-    if (getenv("KS")) best.ksplit = atoi(getenv("KS"));
-    if (getenv("CL")) best.cluster = atoi(getenv("CL"));
-    if (getenv("ST")) best.stages = atoi(getenv("ST"));
-#endif
     const int64_t run = (chunks + best.cluster - 1) / best.cluster;
     best.x_chunks = std::max<int64_t>(1, 16 * 1024 / x_chunk / best.ksplit) * best.ksplit;
     best.x_chunks = std::min<int64_t>(best.x_chunks, (run + best.ksplit - 1) / best.ksplit * best.ksplit);

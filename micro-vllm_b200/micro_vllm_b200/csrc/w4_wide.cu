@@ -1,6 +1,5 @@
 // Plans and launches of the tcgen05 product kernel (w4_wide.cuh), and the device status that its waits set.
 #include <algorithm>
-#include <cstdlib>
 #include <cudaTypedefs.h>
 
 #include <mutex>
@@ -65,9 +64,6 @@ int wide_cluster(int64_t blocks, int chunks, int nt, const int* slots) {
         else time += 5.2 + (2 * blocks <= slots[i] ? run * 0.33 : 2 * rounds * (3.0 + run * 0.22));
         if (c == 1 || time < least) least = time, best = c;
     }
-#ifdef MVQ_TUNE
-    if (getenv("CL")) return atoi(getenv("CL"));
-#endif
     return best;
 }
 
@@ -101,6 +97,9 @@ int launch_one(LinearParams p, int device, int sms, void* stream) {
                 cfg.numAttrs = 1;
                 err = cudaOccupancyMaxActiveClusters(&slots[device][i], kernel, &cfg);
                 if (err != cudaSuccess) return cuda_fail(err, "cudaOccupancyMaxActiveClusters");
+                // It counts one CTA per SM for every kernel that allocates tensor memory, but two of 256
+                // columns do run together (224 CTAs of 16 rows in 21.5 us; made for one per SM, 27.6).
+                slots[device][i] *= Shape::kCtas;
             }
             ready[device] = true;
         }

@@ -42,11 +42,18 @@ struct WideShape {
     static constexpr int kTurns = NT == 64 ? 2 : 1;        // groups of sets that take chunks in turn (NT 128 leaves no threads for it)
     static constexpr int kThreads = (8 + 4 * kSets * kTurns + 2) * 32;
     static constexpr int kCtas = NT <= 32 ? 2 : 1;         // per SM
+    // Fourteen warps fall on the four schedulers as 4 4 3 3, so that two CTAs fit as
+    // sixteen each would, at 64 registers. 32 tokens would spill for that.
+    static constexpr int kBoundThreads = NT == 16 ? 512 : kThreads;
     static constexpr int kStages = NT == 64 ? 5 : 3;       // records in flight per converting warp
     static constexpr int kACols = KIND == kI8 ? 32 : 64;   // TMEM columns of a chunk of A
     static constexpr int kBuffers = NT <= 32 && KIND != kI8 ? 3 : 4;  // chunks of A and of X
     static constexpr int kTmemCols = NT <= 32 ? 256 : 512;
-    static_assert(kBuffers * kACols + 2 * NT <= kTmemCols, "TMEM columns");
+    // Buffers of D: those of two whole chunks where they fit, so that a chunk's arrival
+    // says that its D is free; else two, each group waiting for its own (d_empty).
+    static constexpr bool kWholeChunks = kBuffers * kACols + 2 * kGroups * NT <= kTmemCols;
+    static constexpr int kDBuffers = kWholeChunks ? 2 * kGroups : 2;
+    static_assert(kBuffers * kACols + kDBuffers * NT <= kTmemCols, "TMEM columns");
     static constexpr int kXBytes = NT * (KIND == kI8 ? 128 : 256);
     static constexpr int kStageBytes = kCodeBytes / 2 + (ZEROS ? kGroups * 64 : 0);
     static constexpr int kRings = 8 * kStages * kStageBytes;
@@ -159,7 +166,7 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
 
 // `xmap`: X as [m, k] in boxes of NT rows of 128 bytes, where p.x_units says that it can be copied as it is.
 template <int KIND, int NT, int GROUP, bool ZEROS>
-__global__ void __launch_bounds__(WideShape<KIND, NT, GROUP, ZEROS>::kThreads, WideShape<KIND, NT, GROUP, ZEROS>::kCtas)
+__global__ void __launch_bounds__(WideShape<KIND, NT, GROUP, ZEROS>::kBoundThreads, WideShape<KIND, NT, GROUP, ZEROS>::kCtas)
 w4_wide_kernel(const LinearParams p, const __grid_constant__ CUtensorMap xmap) {
     using A = Act<KIND>;
     using Shape = WideShape<KIND, NT, GROUP, ZEROS>;
@@ -170,9 +177,10 @@ w4_wide_kernel(const LinearParams p, const __grid_constant__ CUtensorMap xmap) {
     extern __shared__ uint8_t smem_raw[];
     // full: a chunk's A and X are in place and D of the chunk two before is
     // drained. done: its last group is multiplied, which frees A and X and hands
-    // over D. part_done and d_empty only serve chunks of several groups; each turn
-    // has its own part_done, since a waiter may not skip a phase of a barrier.
-    __shared__ __align__(8) uint64_t full[kAB], done[kAB], part_done[kTurns][2], d_empty[2], drained;
+    // over D. part_done, for the other groups of chunks of several, has a
+    // barrier for each buffer of D, or, where groups wait for their buffers, two for
+    // each turn: no waiter may skip a phase, and no barrier run two phases ahead.
+    __shared__ __align__(8) uint64_t full[kAB], done[kAB], part_done[2][kGroups > 2 ? kGroups : 2], d_empty[2], drained;
     __shared__ uint32_t s_tmem;
     __shared__ float s_scale[NT], s_bias[kWideRows];
     __shared__ volatile int s_failed;
@@ -206,7 +214,7 @@ w4_wide_kernel(const LinearParams p, const __grid_constant__ CUtensorMap xmap) {
             mv::mbar_init(mv::smem_addr(&done[i]), 1);
         }
         for (int i = 0; i < 2; ++i) {
-            for (int turn = 0; turn < kTurns; ++turn) mv::mbar_init(mv::smem_addr(&part_done[turn][i]), 1);
+            for (int j = 0; j < (kGroups > 2 ? kGroups : 2); ++j) mv::mbar_init(mv::smem_addr(&part_done[i][j]), 1);
             mv::mbar_init(mv::smem_addr(&d_empty[i]), 4 * kSets);
         }
         mv::mbar_init(mv::smem_addr(&drained), 1);
@@ -331,7 +339,7 @@ w4_wide_kernel(const LinearParams p, const __grid_constant__ CUtensorMap xmap) {
 #pragma unroll
             for (int gi = 0; gi < kGroups; ++gi) {
                 const int u = i * kGroups + gi;
-                if (kGroups > 1 && u >= 2) ok = ok && wait(&d_empty[u & 1], (u >> 1) - 1);
+                if (!Shape::kWholeChunks && u >= 2) ok = ok && wait(&d_empty[u & 1], (u >> 1) - 1);
                 if (!ok) break;
                 fence_after();
                 const uint32_t a_at = tmem + (i % kAB) * Shape::kACols + gi * kSteps * 8;
@@ -340,10 +348,12 @@ w4_wide_kernel(const LinearParams p, const __grid_constant__ CUtensorMap xmap) {
                 for (int s = 0; s < kSteps; ++s) {
                     const int step = gi * kSteps + s;
                     const uint32_t b = KIND == kI8 ? x_at + step * 32 : x_at + (step >> 2) * (NT * 128) + (step & 3) * 32;
-                    wide_mma<KIND>(leader, d_col + (u & 1) * NT, a_at + s * 8, sw128_desc(b), wide_idesc<KIND, NT>(), s > 0);
+                    wide_mma<KIND>(leader, d_col + (u % Shape::kDBuffers) * NT, a_at + s * 8, sw128_desc(b), wide_idesc<KIND, NT>(), s > 0);
                 }
                 const int v = i / kTurns * (kGroups - 1) + gi;
-                wide_commit(leader, mv::smem_addr(gi == kGroups - 1 ? &done[i % kAB] : &part_done[i % kTurns][v & 1]));
+                wide_commit(leader, mv::smem_addr(gi == kGroups - 1        ? &done[i % kAB]
+                                                  : Shape::kWholeChunks ? &part_done[i & 1][gi]
+                                                                        : &part_done[i % kTurns][v & 1]));
             }
             if (!ok) break;
         }
@@ -447,16 +457,17 @@ w4_wide_kernel(const LinearParams p, const __grid_constant__ CUtensorMap xmap) {
                 const int u = i * kGroups + gi, v = i / kTurns * (kGroups - 1) + gi;
                 const float2 both = scale_pair(scales[gi], p.scale_bf16);
                 const float sc = lane & 8 ? both.y : both.x;
-                ok = ok && (gi == kGroups - 1 ? wait(&done[i % kAB], i / kAB) : wait(&part_done[turn][v & 1], v >> 1));
+                ok = ok && (gi == kGroups - 1 ? wait(&done[i % kAB], i / kAB)
+                                              : (Shape::kWholeChunks ? wait(&part_done[i & 1][gi], i >> 1) : wait(&part_done[turn][v & 1], v >> 1)));
                 if (!ok) break;
                 fence_after();
-                const uint32_t from = lanes + (u & 1) * NT;
+                const uint32_t from = lanes + (u % Shape::kDBuffers) * NT;
 #pragma unroll
                 for (int c = 0; c < Shape::kCols; c += 16) {
                     uint32_t r[16];
                     tmem_ld_16(from + c, r);
                     wait_ld();
-                    if (kGroups > 1 && c + 16 == Shape::kCols) {
+                    if (!Shape::kWholeChunks && c + 16 == Shape::kCols) {
                         fence_before();
                         __syncwarp();
                         if (lane == 0) wide_arrive(mv::smem_addr(&d_empty[u & 1]));

@@ -40,9 +40,11 @@ from .rope import apply_rope, rope_tables
 from .row_ops import add_rms_norm, add_rms_norm_quant, rms_norm, silu_mul, silu_mul_quant
 from .w4_linear import quantize_w4, w4_dequantize, w4_linear
 
-# Rows up to which 4-bit projections multiply their codes; beyond, the projection
-# is written out first and multiplied by the library. Measured on B200 for 3584 x
-# 28672 in bf16: EXPAND_NOTE
+# Rows of a 16-bit prompt up to which 4-bit projections multiply their codes; beyond,
+# the projection is written out first and multiplied by the library. Measured on B200
+# for 3584 x 28672 in bf16: 128 rows 50 us and 88, 192 rows 90 and 91, 256 rows 99 and
+# 91. In fp32, where the library's product is slow, the codes stay ahead (512 rows
+# 1.59 ms and 1.92): four times as many rows.
 CODES_ROWS = 128
 
 
@@ -140,7 +142,8 @@ class PreparedModel:
         """A projection as a matrix, or None where its codes are multiplied as they are."""
         if self.weight_bits == 16:
             return w[name]
-        return None if rows <= CODES_ROWS else w4_dequantize(w[name], self.dtype)
+        most = CODES_ROWS * (4 if self.dtype == torch.float32 else 1)
+        return None if rows <= most else w4_dequantize(w[name], self.dtype)
 
     def _project(self, x, w, name, bias=None, residual=None):
         """x [..., in] through a projection, + bias or + residual (of the output's shape)."""
