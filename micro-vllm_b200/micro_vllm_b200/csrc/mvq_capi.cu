@@ -22,6 +22,7 @@ int fail(int code, const char* fmt, ...) {
 }
 
 int cuda_fail(cudaError_t err, const char* what) {
+    cudaGetLastError();  // reported here: not once more by whoever asks the runtime next
     return fail(MVQ_ERR_CUDA, "%s: %s", what, cudaGetErrorString(err));
 }
 
@@ -55,10 +56,13 @@ int device_sms(int* device, int* sms) {
 bool float_dtype(int64_t d) { return d == MVQ_DTYPE_F32 || d == MVQ_DTYPE_F16 || d == MVQ_DTYPE_BF16; }
 int64_t dtype_size(int64_t d) { return d == MVQ_DTYPE_F32 ? 4 : d == MVQ_DTYPE_F16 || d == MVQ_DTYPE_BF16 ? 2 : 1; }
 uintptr_t address(const void* p) { return reinterpret_cast<uintptr_t>(p); }
+bool off_element(const void* p, int64_t dtype) { return address(p) % dtype_size(dtype) != 0; }
 
 // ------------------------------------------------------------------- weights
 
 constexpr int64_t kMaxSize = int64_t(1) << 30;
+// Rows of x per launch: a grid's 65535 blocks of the narrow kernel's eight.
+constexpr int64_t kLaunchRows = int64_t(65535) * mvq::kTokens;
 
 int check_weight(const void* records, int64_t n, int64_t k, int64_t group, int64_t scale_dtype) {
     if (!records) return fail(MVQ_ERR_INVALID_ARGUMENT, "records must not be NULL");
@@ -171,34 +175,31 @@ int mvq_w4_linear(const MvqLinearArgs* a, void* stream) try {
         return fail(MVQ_ERR_INVALID_ARGUMENT, "out_dtype must be MVQ_DTYPE_F32, MVQ_DTYPE_F16 or MVQ_DTYPE_BF16");
     if (a->m > 1 && (a->x_stride_row < 0 || a->out_stride_row < a->n || (a->residual && a->residual_stride_row < 0)))
         return fail(MVQ_ERR_INVALID_ARGUMENT, "row strides must be nonnegative and out's rows must not overlap");
+    if (off_element(a->x, a->x_dtype) || off_element(a->x_scale, MVQ_DTYPE_F32) || off_element(a->bias, a->out_dtype) ||
+        off_element(a->residual, a->out_dtype) || off_element(a->out, a->out_dtype))
+        return fail(MVQ_ERR_INVALID_ARGUMENT, "pointers must be aligned to their elements");
     int device, sms;
     rc = device_sms(&device, &sms);
     if (rc != MVQ_OK) return rc;
     const int64_t size = dtype_size(a->x_dtype);
     const int64_t run = size == 1 ? 8 : 16;  // bytes of a vector load of x
     mvq::LinearParams p = {};
-    p.x = a->x;
     p.x_stride = a->x_stride_row;
-    p.x_scale = static_cast<const float*>(a->x_scale);
     p.records = static_cast<const uint8_t*>(a->records);
     p.n = static_cast<int>(a->n);
     p.k = static_cast<int>(a->k);
-    p.m = static_cast<int>(a->m);
     p.chunks = static_cast<int>((a->k + mvq::kChunk - 1) / mvq::kChunk);
     p.tiles = static_cast<int>((a->n + mvq::kTileRows - 1) / mvq::kTileRows);
     p.x_dtype = static_cast<int>(a->x_dtype);
     p.scale_bf16 = a->scale_dtype == MVQ_DTYPE_BF16;
     p.x_runs = a->k % 8 == 0 && address(a->x) % run == 0 && (a->m == 1 || a->x_stride_row * size % run == 0);
     p.bias = a->bias;
-    p.residual = a->residual;
     p.residual_stride = a->residual_stride_row;
-    p.out = a->out;
     p.out_stride = a->out_stride_row;
     p.out_dtype = static_cast<int>(a->out_dtype);
     // TMA wants 16-byte rows that do not overlap.
     p.x_units = (size == 2 || a->x_dtype == MVQ_DTYPE_I8) && address(a->x) % 16 == 0 &&
-                (a->m == 1 || (a->x_stride_row * size % 16 == 0 && a->x_stride_row >= a->k &&
-                               a->x_stride_row < (int64_t(1) << 38)));
+                a->x_stride_row * size % 16 == 0 && a->x_stride_row >= a->k && a->x_stride_row < (int64_t(1) << 38);
     const int kind = a->x_dtype == MVQ_DTYPE_E4M3 ? mvq::kF16 : static_cast<int>(a->x_dtype);
     const int group = static_cast<int>(a->group);
     // The mma.sync kernel up to eight rows, except for five to eight rows of small
@@ -207,9 +208,20 @@ int mvq_w4_linear(const MvqLinearArgs* a, void* stream) try {
     // int8 14.7 and 13.4; 3584 x 28672 in bf16 21.4 both, in int8 18.0 and 15.6).
     const bool small = p.chunks <= 16 || (kind != mvq::kI8 && p.tiles <= 64);
     const int few = small ? 4 : 8;
-    if (kind == mvq::kF32 || a->m <= few)
-        return mvq::launch_narrow(p, kind, group, a->has_zeros != 0, device, sms, stream);
-    return mvq::launch_wide(p, kind, group, a->has_zeros != 0, device, sms, stream);
+    const int64_t out_size = dtype_size(a->out_dtype);
+    for (int64_t m0 = 0; m0 < a->m; m0 += kLaunchRows) {
+        p.m = static_cast<int>(a->m - m0 < kLaunchRows ? a->m - m0 : kLaunchRows);
+        p.x = static_cast<const uint8_t*>(a->x) + m0 * a->x_stride_row * size;
+        if (a->x_scale) p.x_scale = static_cast<const float*>(a->x_scale) + m0;
+        if (a->residual)
+            p.residual = static_cast<const uint8_t*>(a->residual) + m0 * a->residual_stride_row * out_size;
+        p.out = static_cast<uint8_t*>(a->out) + m0 * a->out_stride_row * out_size;
+        rc = kind == mvq::kF32 || p.m <= few
+                 ? mvq::launch_narrow(p, kind, group, a->has_zeros != 0, device, sms, stream)
+                 : mvq::launch_wide(p, kind, group, a->has_zeros != 0, device, sms, stream);
+        if (rc != MVQ_OK) return rc;
+    }
+    return MVQ_OK;
 } catch (...) {
     return fail(MVQ_ERR_CUDA, "unexpected C++ exception");
 }
@@ -223,6 +235,8 @@ int mvq_w4_dequantize(const MvqDequantizeArgs* a, void* stream) try {
         return fail(MVQ_ERR_INVALID_ARGUMENT, "out_dtype must be MVQ_DTYPE_F32, MVQ_DTYPE_F16 or MVQ_DTYPE_BF16");
     if (a->n > 1 && a->out_stride_row < a->k)
         return fail(MVQ_ERR_INVALID_ARGUMENT, "out's rows must not overlap");
+    if (off_element(a->out, a->out_dtype))
+        return fail(MVQ_ERR_INVALID_ARGUMENT, "pointers must be aligned to their elements");
     const int chunks = static_cast<int>((a->k + mvq::kChunk - 1) / mvq::kChunk);
     const int64_t total = (a->n + mvq::kTileRows - 1) / mvq::kTileRows * chunks;
     if (total >= (int64_t(1) << 31)) return fail(MVQ_ERR_UNSUPPORTED, "the weight is too large for one call");
@@ -265,6 +279,10 @@ int mvq_add_rms_norm(const MvqNormArgs* a, void* stream) try {
                         a->out_stride_row < a->hidden ||
                         (a->residual_out && a->residual_out_stride_row < a->hidden)))
         return fail(MVQ_ERR_INVALID_ARGUMENT, "row strides must be nonnegative and outputs' rows must not overlap");
+    if (off_element(a->x, a->dtype) || off_element(a->residual, a->dtype) || off_element(a->weight, a->dtype) ||
+        off_element(a->residual_out, a->dtype) || off_element(a->out, a->out_dtype) ||
+        off_element(a->scales, MVQ_DTYPE_F32))
+        return fail(MVQ_ERR_INVALID_ARGUMENT, "pointers must be aligned to their elements");
     int device, sms;
     rc = device_sms(&device, &sms);
     if (rc != MVQ_OK) return rc;
@@ -313,6 +331,8 @@ int mvq_silu_mul_quant(const MvqSiluArgs* a, void* stream) try {
         return fail(MVQ_ERR_INVALID_ARGUMENT, "out_dtype must be MVQ_DTYPE_I8 or MVQ_DTYPE_E4M3");
     if (a->rows > 1 && (a->stride_row < 0 || a->out_stride_row < a->width))
         return fail(MVQ_ERR_INVALID_ARGUMENT, "row strides must be nonnegative and out's rows must not overlap");
+    if (off_element(a->gate_up, a->dtype) || off_element(a->scales, MVQ_DTYPE_F32))
+        return fail(MVQ_ERR_INVALID_ARGUMENT, "pointers must be aligned to their elements");
     int device, sms;
     rc = device_sms(&device, &sms);
     if (rc != MVQ_OK) return rc;

@@ -73,7 +73,6 @@ int launch_linear(LinearParams p, const LinearPlan& plan, int device, void* stre
         }
     }
     const int64_t blocks = (static_cast<int64_t>(p.m) + kTokens - 1) / kTokens;
-    if (blocks > 65535) return fail(MVQ_ERR_UNSUPPORTED, "too many rows of x for one call");
     const int per_cta = kWarps / plan.ksplit;
     const int64_t ctas = (static_cast<int64_t>(p.tiles) + per_cta - 1) / per_cta * plan.cluster;
     if (ctas >= (int64_t(1) << 31)) return fail(MVQ_ERR_UNSUPPORTED, "too many weight rows for one call");

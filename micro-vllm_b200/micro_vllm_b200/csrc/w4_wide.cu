@@ -29,7 +29,7 @@ int x_map(const LinearParams& p, int kind, int rows, CUtensorMap* map) {
     if (!encode) return fail(MVQ_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable from the driver");
     const int size = kind == kI8 ? 1 : 2;
     const cuuint64_t dims[2] = {static_cast<cuuint64_t>(p.k), static_cast<cuuint64_t>(p.m)};
-    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(p.m == 1 ? (p.k * size + 15) / 16 * 16 : p.x_stride * size)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(p.x_stride * size)};
     const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / size), static_cast<cuuint32_t>(rows)};
     const cuuint32_t steps[2] = {1, 1};
     const CUresult r = encode(map, kind == kI8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
@@ -106,7 +106,6 @@ int launch_one(LinearParams p, int device, int sms, void* stream) {
     }
     const int64_t blocks = (static_cast<int64_t>(p.n) + kWideRows - 1) / kWideRows;
     const int64_t passes = (static_cast<int64_t>(p.m) + NT - 1) / NT;
-    if (passes > 65535) return fail(MVQ_ERR_UNSUPPORTED, "too many rows of x for one call");
     p.cluster = wide_cluster(blocks * passes, p.chunks, NT, slots[device]);
     CUtensorMap map = {};
     if (p.x_units) {

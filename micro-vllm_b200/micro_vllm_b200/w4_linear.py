@@ -60,6 +60,10 @@ class W4Weight:
     def nbytes(self):
         return self.records.numel()
 
+    def __reduce__(self):
+        # A copy's addresses are those of its own records.
+        return W4Weight, (self.records, self.shape, self.group_size, self.has_zeros, self.scale_dtype)
+
     def to(self, device):
         """This weight on another device (itself where it is there already)."""
         records = self.records.to(device)

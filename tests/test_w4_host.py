@@ -180,3 +180,52 @@ def test_import_loads_no_native_code_and_a_missing_library_fails_loudly(tmp_path
             _quant_native.library()
     finally:
         _quant_native.library.cache_clear()
+
+
+def test_copies_of_a_weight_point_at_their_own_records():
+    import copy
+    import pickle
+
+    from micro_vllm_b200.w4_linear import pack_w4
+    codes, scales, zero = checkpoint(70, 130, 64, True, torch.float16, seed=3)
+    weight = pack_w4(codes, scales, zero, group_size=64)
+    for other in (copy.copy(weight), copy.deepcopy(weight), pickle.loads(pickle.dumps(weight))):
+        assert torch.equal(other.records, weight.records) and repr(other) == repr(weight)
+        assert other.fixed == (other.records.data_ptr(), *weight.fixed[1:]) and other.index == weight.index
+    assert copy.deepcopy(weight).fixed[0] != weight.fixed[0]
+
+
+def test_checkpoints_may_be_strided():
+    from micro_vllm_b200.w4_linear import pack_w4, quantize_w4
+    codes, scales, _ = checkpoint(128, 256, 64, False, torch.float16, seed=4)
+    kept = codes.clone()
+    records = pack_w4(codes, scales, group_size=64).records
+    assert torch.equal(codes, kept)
+    strided = pack_w4(codes.t().contiguous().t(), scales.t().contiguous().t(), group_size=64)
+    assert torch.equal(strided.records, records)
+    one = pack_w4(codes[:1].expand(128, 256), scales[:1].expand(128, 4), group_size=64)
+    assert torch.equal(one.records, pack_w4(codes[:1].repeat(128, 1), scales[:1].repeat(128, 1), group_size=64).records)
+    matrix = torch.randn((128, 256), generator=torch.Generator().manual_seed(5))
+    assert torch.equal(quantize_w4(matrix.t().contiguous().t()).records, quantize_w4(matrix).records)
+
+
+def test_pointers_off_their_elements_are_refused_without_a_gpu():
+    from micro_vllm_b200 import _native, _quant_native as q
+    lib = _library()
+    linear = dict(x=64, x_stride_row=128, x_scale=0, records=64, n=64, k=128, group=128, has_zeros=0,
+                  scale_dtype=q.DTYPE_BF16, bias=0, residual=0, residual_stride_row=0, out=64, out_stride_row=64, m=2,
+                  x_dtype=q.DTYPE_BF16, out_dtype=q.DTYPE_F32)
+    norm = dict(x=64, x_stride_row=8, residual=0, residual_stride_row=0, weight=64, out=64, out_stride_row=8, scales=64,
+                residual_out=0, residual_out_stride_row=0, rows=2, hidden=8, eps=1e-6, dtype=2, out_dtype=3)
+    silu = dict(gate_up=64, stride_row=16, out=64, out_stride_row=8, scales=64, rows=2, width=8, dtype=0, out_dtype=3)
+    deq = dict(records=64, n=64, k=128, group=32, has_zeros=0, scale_dtype=1, out=64, out_stride_row=128, out_dtype=0)
+    for entry, pack, names, good, bad in [
+        (lib.mvq_w4_linear, q.pack_linear, q.LINEAR_FIELDS, linear,
+         dict(x=65, x_scale=66, bias=66, residual=66, out=66)),
+        (lib.mvq_add_rms_norm, q.pack_norm, q.NORM_FIELDS, norm, dict(x=65, residual=65, weight=65, scales=66)),
+        (lib.mvq_silu_mul_quant, q.pack_silu, q.SILU_FIELDS, silu, dict(gate_up=66, scales=66)),
+        (lib.mvq_w4_dequantize, q.pack_dequantize, q.DEQUANTIZE_FIELDS, deq, dict(out=66)),
+    ]:
+        for name, value in bad.items():
+            with pytest.raises(_native.NativeError, match='aligned to their elements'):
+                q.check(entry(pack(*({**good, name: value}[f] for f in names)), None))
