@@ -198,8 +198,8 @@ int mvq_w4_linear(const MvqLinearArgs* a, void* stream) try {
     p.out_stride = a->out_stride_row;
     p.out_dtype = static_cast<int>(a->out_dtype);
     // TMA wants 16-byte rows that do not overlap.
-    p.x_units = (size == 2 || a->x_dtype == MVQ_DTYPE_I8) && address(a->x) % 16 == 0 &&
-                a->x_stride_row * size % 16 == 0 && a->x_stride_row >= a->k && a->x_stride_row < (int64_t(1) << 38);
+    p.x_units = size < 4 && address(a->x) % 16 == 0 && a->x_stride_row * size % 16 == 0 && a->x_stride_row >= a->k &&
+                a->x_stride_row < (int64_t(1) << 38);
     const int kind = a->x_dtype == MVQ_DTYPE_E4M3 ? mvq::kF16 : static_cast<int>(a->x_dtype);
     const int group = static_cast<int>(a->group);
     // The mma.sync kernel up to eight rows, except for five to eight rows of small
@@ -218,7 +218,7 @@ int mvq_w4_linear(const MvqLinearArgs* a, void* stream) try {
         p.out = static_cast<uint8_t*>(a->out) + m0 * a->out_stride_row * out_size;
         rc = kind == mvq::kF32 || p.m <= few
                  ? mvq::launch_narrow(p, kind, group, a->has_zeros != 0, device, sms, stream)
-                 : mvq::launch_wide(p, kind, group, a->has_zeros != 0, device, sms, stream);
+                 : mvq::launch_wide(p, p.x_dtype, group, a->has_zeros != 0, device, sms, stream);
         if (rc != MVQ_OK) return rc;
     }
     return MVQ_OK;

@@ -41,7 +41,7 @@ cudaError_t launch(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem
 }
 
 // p as w4_linear.cuh's kernels take it, without the fields that a plan sets.
-// `kind`: kF32, kF16 (e4m3 rows too), kBF16 or kI8.
+// `kind`: kF32, kF16, kBF16 or kI8; e4m3 rows are kF16 to the narrow kernel, kE4M3 to the wide one.
 int launch_narrow(const LinearParams& p, int kind, int group, bool zeros, int device, int sms, void* stream);
 int launch_wide(const LinearParams& p, int kind, int group, bool zeros, int device, int sms, void* stream);
 

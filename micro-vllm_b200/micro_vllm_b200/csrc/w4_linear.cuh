@@ -52,7 +52,7 @@ struct LinearParams {
     int scale_bf16;
     int x_dtype;
     int x_runs;        // x may be read 8 elements at a time: aligned rows, k a multiple of 8
-    int x_units;       // x may be copied in units of 16 bytes as it is
+    int x_units;       // x's rows may be copied by TMA
     int cluster;       // CTAs that share a tile's columns, each with a run of chunks
     int ksplit;        // warps of a CTA that share a tile's columns: its kWarps / ksplit tiles
     int stages;        // records in flight per warp
@@ -215,6 +215,13 @@ __device__ __forceinline__ void mma_s8(int (&c)[4], const uint32_t (&a)[4], uint
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// Four e4m3 numbers as fp16, exactly.
+__device__ __forceinline__ uint2 e4m3_to_half(uint32_t v) {
+    const __half2_raw lo = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(v & 0xffffu), __NV_E4M3);
+    const __half2_raw hi = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(v >> 16), __NV_E4M3);
+    return make_uint2(lo.x | (static_cast<uint32_t>(lo.y) << 16), hi.x | (static_cast<uint32_t>(hi.y) << 16));
+}
+
 // Eight consecutive elements of a row of x, columns k..k+7 (zeros at and beyond
 // `limit`), as operand numbers of kind KIND: r[plane][...] holds them in order,
 // two to a register (int8: four). e4m3 numbers are exact in fp16.
@@ -275,12 +282,8 @@ __device__ __forceinline__ void load_run(const LinearParams& p, const void* row,
         if constexpr (KIND == kI8) {
             r[0][0] = v.x, r[0][1] = v.y;
         } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t pair = (i < 2 ? v.x : v.y) >> (16 * (i & 1)) & 0xffffu;
-                const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(pair), __NV_E4M3);
-                r[0][i] = h.x | (static_cast<uint32_t>(h.y) << 16);
-            }
+            const uint2 lo = e4m3_to_half(v.x), hi = e4m3_to_half(v.y);
+            r[0][0] = lo.x, r[0][1] = lo.y, r[0][2] = hi.x, r[0][3] = hi.y;
         }
     }
 }

@@ -23,19 +23,19 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     return fn;
 }
 
-// X as [m, k] in boxes of `rows` rows of 128 bytes, swizzled; what lies beyond reads as zero.
+// X as [m, k] in boxes of `rows` rows of 128 bytes, swizzled (e4m3 rows as they lie); what lies beyond reads as zero.
 int x_map(const LinearParams& p, int kind, int rows, CUtensorMap* map) {
     auto encode = encode_fn();
     if (!encode) return fail(MVQ_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable from the driver");
-    const int size = kind == kI8 ? 1 : 2;
+    const int size = kind == kI8 || kind == kE4M3 ? 1 : 2;
     const cuuint64_t dims[2] = {static_cast<cuuint64_t>(p.k), static_cast<cuuint64_t>(p.m)};
     const cuuint64_t strides[1] = {static_cast<cuuint64_t>(p.x_stride * size)};
     const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / size), static_cast<cuuint32_t>(rows)};
     const cuuint32_t steps[2] = {1, 1};
-    const CUresult r = encode(map, kind == kI8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+    const CUresult r = encode(map, size == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                    : kind == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                               2, const_cast<void*>(p.x), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              kind == kE4M3 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(MVQ_ERR_CUDA, "cuTensorMapEncodeTiled failed (CUresult %d)", static_cast<int>(r));
     return MVQ_OK;
@@ -192,6 +192,7 @@ int launch_wide(const LinearParams& p, int kind, int group, bool zeros, int devi
     switch (kind) {
         case kBF16: return launch_kind<kBF16>(p, group, zeros, device, sms, stream);
         case kI8: return launch_kind<kI8>(p, group, zeros, device, sms, stream);
+        case kE4M3: return launch_kind<kE4M3>(p, group, zeros, device, sms, stream);
         default: return launch_kind<kF16>(p, group, zeros, device, sms, stream);
     }
 }

@@ -57,7 +57,8 @@ struct WideShape {
     static constexpr int kXBytes = NT * (KIND == kI8 ? 128 : 256);
     static constexpr int kStageBytes = kCodeBytes / 2 + (ZEROS ? kGroups * 64 : 0);
     static constexpr int kRings = 8 * kStages * kStageBytes;
-    static constexpr int kUsed = kBuffers * kXBytes + kRings;
+    static constexpr int kRawBytes = KIND == kE4M3 ? NT * 128 : 0;  // a chunk of e4m3 rows, before it is fp16
+    static constexpr int kUsed = kBuffers * kXBytes + kRings + 2 * kRawBytes;
     static constexpr int kPart = kTurns * NT * kWidePartStride * 4;
     static constexpr int kSmem = (kUsed > kPart ? kUsed : kPart) + 1024;
 };
@@ -77,7 +78,8 @@ __device__ __forceinline__ uint32_t elect_one() {
 // D fp32 (1) or s32 (2); A and B fp16 (0), bf16 (1) or s8 (1); both K-major.
 template <int KIND, int NT>
 __host__ __device__ constexpr uint32_t wide_idesc() {
-    return ((KIND == kI8 ? 2u : 1u) << 4) | ((KIND == kF16 ? 0u : 1u) << 7) | ((KIND == kF16 ? 0u : 1u) << 10) |
+    constexpr uint32_t kHalf = KIND == kF16 || KIND == kE4M3 ? 0u : 1u;
+    return ((KIND == kI8 ? 2u : 1u) << 4) | (kHalf << 7) | (kHalf << 10) |
            (static_cast<uint32_t>(NT >> 3) << 17) | (static_cast<uint32_t>(kWideRows >> 4) << 24);
 }
 
@@ -168,7 +170,8 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
 template <int KIND, int NT, int GROUP, bool ZEROS>
 __global__ void __launch_bounds__(WideShape<KIND, NT, GROUP, ZEROS>::kBoundThreads, WideShape<KIND, NT, GROUP, ZEROS>::kCtas)
 w4_wide_kernel(const LinearParams p, const __grid_constant__ CUtensorMap xmap) {
-    using A = Act<KIND>;
+    constexpr int kOperand = KIND == kE4M3 ? kF16 : KIND;  // e4m3 rows become fp16
+    using A = Act<kOperand>;
     using Shape = WideShape<KIND, NT, GROUP, ZEROS>;
     constexpr int kGroups = Shape::kGroups;
     constexpr int kRecord = record_size(GROUP, ZEROS);
@@ -180,7 +183,7 @@ w4_wide_kernel(const LinearParams p, const __grid_constant__ CUtensorMap xmap) {
     // over D. part_done, for the other groups of chunks of several, has a
     // barrier for each buffer of D, or, where groups wait for their buffers, two for
     // each turn: no waiter may skip a phase, and no barrier run two phases ahead.
-    __shared__ __align__(8) uint64_t full[kAB], done[kAB], part_done[2][kGroups > 2 ? kGroups : 2], d_empty[2], drained;
+    __shared__ __align__(8) uint64_t full[kAB], done[kAB], part_done[2][kGroups > 2 ? kGroups : 2], d_empty[2], raw_full[2], drained;
     __shared__ uint32_t s_tmem;
     __shared__ float s_scale[NT], s_bias[kWideRows];
     __shared__ volatile int s_failed;
@@ -197,6 +200,8 @@ w4_wide_kernel(const LinearParams p, const __grid_constant__ CUtensorMap xmap) {
         reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     const uint32_t xs = mv::smem_addr(smem);
     const uint32_t rings = xs + kAB * Shape::kXBytes;
+    const uint32_t raws = rings + Shape::kRings;
+    const bool raw = KIND == kE4M3 && p.x_units;  // x comes by TMA, but is not fp16 yet
 
     // A converting or draining warp w has rows 32 (w % 4).. of the 128: half p = w & 1
     // of tile (w % 4) >> 1. A second tile beyond the weight's last reads the
@@ -216,6 +221,7 @@ w4_wide_kernel(const LinearParams p, const __grid_constant__ CUtensorMap xmap) {
         for (int i = 0; i < 2; ++i) {
             for (int j = 0; j < (kGroups > 2 ? kGroups : 2); ++j) mv::mbar_init(mv::smem_addr(&part_done[i][j]), 1);
             mv::mbar_init(mv::smem_addr(&d_empty[i]), 4 * kSets);
+            mv::mbar_init(mv::smem_addr(&raw_full[i]), 1);
         }
         mv::mbar_init(mv::smem_addr(&drained), 1);
         s_failed = 0;
@@ -365,9 +371,15 @@ w4_wide_kernel(const LinearParams p, const __grid_constant__ CUtensorMap xmap) {
         bool ok = true;
         for (int i = 0; i < n && ok; ++i) {
             if (i >= kAB) ok = wait(&done[i % kAB], i / kAB - 1);
+            if (raw && i >= 2) ok = ok && wait(&full[(i - 2) % kAB], (i - 2) / kAB);  // its raw rows are read
             if (leader && ok) {
                 const uint32_t bar = mv::smem_addr(&full[i % kAB]);
-                if (p.x_units) {
+                if (raw) {
+                    const uint32_t raw_bar = mv::smem_addr(&raw_full[i & 1]);
+                    mv::mbar_arrive_expect_tx(raw_bar, Shape::kRawBytes);
+                    tma_load_2d(raws + (i & 1) * Shape::kRawBytes, &xmap, (begin + i) * kChunk, token0, raw_bar);
+                    wide_arrive(bar);
+                } else if (p.x_units) {
                     mv::mbar_arrive_expect_tx(bar, Shape::kXBytes);
                     const uint32_t dst = xs + (i % kAB) * Shape::kXBytes;
                     const int k = (begin + i) * kChunk;
@@ -401,12 +413,34 @@ w4_wide_kernel(const LinearParams p, const __grid_constant__ CUtensorMap xmap) {
                 if (i < n)
                     w[gi] = __ldg(reinterpret_cast<const uint32_t*>(scale + static_cast<int64_t>(i) * kRecord + gi * 128));
         };
-        // X that TMA cannot copy as it is (rows off a 16-byte boundary, e4m3 numbers
-        // that become fp16): these warps store it, element by element at worst.
+        // X that TMA cannot copy as it is: these warps store it, element by element at
+        // worst (rows off a 16-byte boundary). e4m3 numbers that become fp16 come by TMA
+        // into a buffer of their own first (3584 x 28672: 27 us at 16 rows and 53 at 64;
+        // loaded here from global memory, 33 and 78; fp16 rows take 20 and 36).
+        constexpr int kUnits = KIND == kI8 ? 8 : 16;  // 16-byte units of a token's chunk
+        const auto place = [&](uint32_t dst, int token, int unit, const uint4& v) {
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(
+                             dst + (unit >> 3) * (NT * 128) + token * 128 + (((unit & 7) ^ (token & 7)) << 4)),
+                         "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                         : "memory");
+        };
         const auto store_x = [&](int i) {
-            constexpr int kUnits = KIND == kI8 ? 8 : 16;  // 16-byte units of a token's chunk
             const int x_size = p.x_dtype >= kI8 ? 1 : 2;
             const uint32_t dst = xs + (i % kAB) * Shape::kXBytes;
+            if (raw) {
+                if (!wait(&raw_full[i & 1], i >> 1)) return false;
+#pragma unroll 2
+                for (int u = lt; u < NT * kUnits; u += kDrainers) {
+                    uint32_t a, b;
+                    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
+                                 : "=r"(a), "=r"(b)
+                                 : "r"(raws + (i & 1) * Shape::kRawBytes + u * 8));
+                    const uint2 lo = e4m3_to_half(a), hi = e4m3_to_half(b);
+                    place(dst, u / kUnits, u % kUnits, make_uint4(lo.x, lo.y, hi.x, hi.y));
+                }
+                mv::fence_proxy_async_smem();
+                return true;
+            }
 #pragma unroll 1
             for (int u = lt; u < NT * kUnits; u += kDrainers) {
                 const int token = u / kUnits, unit = u % kUnits;
@@ -415,38 +449,36 @@ w4_wide_kernel(const LinearParams p, const __grid_constant__ CUtensorMap xmap) {
                 const uint8_t* row = static_cast<const uint8_t*>(p.x) + (token0 + token) * p.x_stride * x_size;
                 uint32_t r[1][A::kRunBytes / 4];
                 uint4 v;
-                load_run<KIND>(p, row, k, limit, r);
+                load_run<kOperand>(p, row, k, limit, r);
                 if constexpr (KIND == kI8) {
                     v.x = r[0][0], v.y = r[0][1];
-                    load_run<KIND>(p, row, k + 8, limit, r);
+                    load_run<kOperand>(p, row, k + 8, limit, r);
                     v.z = r[0][0], v.w = r[0][1];
                 } else {
                     v = make_uint4(r[0][0], r[0][1], r[0][2], r[0][3]);
                 }
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(
-                                 dst + (unit >> 3) * (NT * 128) + token * 128 + (((unit & 7) ^ (token & 7)) << 4)),
-                             "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
-                             : "memory");
+                place(dst, token, unit, v);
             }
             mv::fence_proxy_async_smem();
+            return true;
         };
         float acc[Shape::kCols];
 #pragma unroll
         for (int e = 0; e < Shape::kCols; ++e) acc[e] = 0.0f;
         const uint32_t lanes = d_col + set * Shape::kCols + (static_cast<uint32_t>(quarter * 32) << 16);
         const auto publish = [&](int i) {  // chunk i may be multiplied, as far as these warps go
-            if (i >= n) return;
-            if (!p.x_units) store_x(i);
+            if (i >= n) return true;
+            if ((raw || !p.x_units) && !store_x(i)) return false;
             fence_before();
             __syncwarp();
             if (lane == 0) wide_arrive(mv::smem_addr(&full[i % kAB]));
+            return true;
         };
         uint32_t scales[kGroups] = {}, scales1[kGroups] = {}, scales2[kGroups] = {};
         load_scales(turn, scales);
         load_scales(turn + kTurns, scales1);
-        publish(turn);
-        if (kTurns == 1) publish(1);
-        bool ok = true;
+        bool ok = publish(turn);
+        if (kTurns == 1) ok = ok && publish(1);
         for (int i = turn; i < n && ok; i += kTurns) {
             load_scales(i + 2 * kTurns, scales2);
             if (lane < kGroups && i + 6 < n)  // the scales come from memory: into L2 well before
@@ -482,7 +514,7 @@ w4_wide_kernel(const LinearParams p, const __grid_constant__ CUtensorMap xmap) {
                 }
             }
             if (!ok) break;
-            publish(i + 2);  // D of chunk i is in registers
+            ok = publish(i + 2);  // D of chunk i is in registers
 #pragma unroll
             for (int gi = 0; gi < kGroups; ++gi) scales[gi] = scales1[gi], scales1[gi] = scales2[gi];
         }
