@@ -202,12 +202,14 @@ int mvq_w4_linear(const MvqLinearArgs* a, void* stream) try {
                 a->x_stride_row < (int64_t(1) << 38);
     const int kind = a->x_dtype == MVQ_DTYPE_E4M3 ? mvq::kF16 : static_cast<int>(a->x_dtype);
     const int group = static_cast<int>(a->group);
-    // The mma.sync kernel up to eight rows, except for five to eight rows of small
-    // weights, where staging x and joining sums outweigh the stream (measured at eight:
-    // 896 x 1152 3.6 to 4.0 us wide, 6.0 narrow; 14336 x 3584 in bf16 15.1 and 17.3, in
-    // int8 14.7 and 13.4; 3584 x 28672 in bf16 21.4 both, in int8 18.0 and 15.6).
+    // The mma.sync kernel for few rows, whose number depends on what staging x and
+    // joining sums cost beside the stream of the weights. Measured (us, wide and
+    // narrow): 896 x 1152 in bf16 at four rows 3.8 and 4.2, at five 3.8 and 5.4; 3584 x
+    // 3584 at four 6.5 and 6.2, at eight 6.3 and 8.8; 3584 x 28672 in bf16 at five 19.7 and
+    // 19.1, at eight 20.1 and 21.3, in int8 at eight 17.4 and 15.7; 14336 x 3584 in int8 at
+    // eight 14.3 and 13.3.
     const bool small = p.chunks <= 16 || (kind != mvq::kI8 && p.tiles <= 64);
-    const int few = small ? 4 : 8;
+    const int few = small ? 4 : kind == mvq::kI8 ? 8 : 6;
     const int64_t out_size = dtype_size(a->out_dtype);
     for (int64_t m0 = 0; m0 < a->m; m0 += kLaunchRows) {
         p.m = static_cast<int>(a->m - m0 < kLaunchRows ? a->m - m0 : kLaunchRows);

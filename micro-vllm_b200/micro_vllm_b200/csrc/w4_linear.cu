@@ -10,7 +10,7 @@ namespace {
 // How a call is cut up (see w4_linear_kernel).
 struct LinearPlan {
     int ksplit, cluster, stages;
-    int64_t x_chunks;
+    int64_t x_bytes, x_chunks;
     size_t ring_bytes, smem;
 };
 
@@ -20,12 +20,16 @@ struct LinearPlan {
 // warp's own latency. The constants (us) are fitted to measured calls of 896 x
 // 1152 to 8192 x 57344 at 1 to 8 tokens: at one token four warps per tile are
 // best (3584 x 28672: 16.2 us, one warp per tile 17.7), at eight one warp per
-// tile and clusters, which share the staged x (21.7 and 28 us).
+// tile and clusters, which share the staged x (21.7 and 28 us). fp32 rows cost
+// mostly their staging as three planes (3584 x 4608 at five tokens: one warp per
+// tile in eights 11.3 us, four warps per tile in eights 14.3). Where few CTAs
+// share an SM, x is staged in one turn or few: 14336 x 3584 in fp32 at eight
+// tokens 25.4 us, 16 KB at a time 40.6.
 LinearPlan linear_plan(int64_t m, int64_t chunks, int64_t tiles, int kind, int record, int sms) {
     const int64_t tokens = std::min<int64_t>(m, kTokens);
     const int64_t blocks = (m + kTokens - 1) / kTokens;
     const int64_t x_chunk = tokens * (kind == kF32 ? 768 : kind == kI8 ? 128 : 256);
-    const double chunk = kind == kI8 ? 0.06 + 0.004 * tokens : kind == kF32 ? 0.25 : 0.11 + 0.007 * tokens;
+    const double chunk = kind == kI8 ? 0.06 + 0.004 * tokens : kind == kF32 ? 0.09 : 0.11 + 0.007 * tokens;
     LinearPlan best = {};
     double least = 0.0;
     for (int ksplit = 1; ksplit <= kWarps; ksplit *= 2) {
@@ -34,20 +38,21 @@ LinearPlan linear_plan(int64_t m, int64_t chunks, int64_t tiles, int kind, int r
             const int64_t run = (chunks + cluster - 1) / cluster;
             const int64_t per_warp = (run + ksplit - 1) / ksplit;
             const double per_sm = static_cast<double>((groups * cluster * blocks + sms - 1) / sms);
-            const double start = 0.7 + 0.006 * tokens * run + 0.02 * tokens;
+            const double start = kind == kF32 ? 0.4 + 0.074 * tokens * run : 0.7 + 0.006 * tokens * run + 0.02 * tokens;
             const double busy = kWarps * std::min(per_sm, 4.0);
             const double time = per_sm * (start + kWarps * per_warp * chunk * std::max(1.0, 12.0 / busy)) +
-                                (cluster > 1 ? 0.6 : 0.0);
+                                (cluster > 1 ? kind == kF32 ? 0.15 * cluster : 0.6 : 0.0);
             if (best.cluster == 0 || time < least) {
                 least = time;
                 best.ksplit = ksplit;
                 best.cluster = cluster;
                 best.stages = per_sm >= 4.0 ? 2 : 3;  // four CTAs per SM, or deeper rings
+                best.x_bytes = (per_sm >= 3.0 ? 16 : per_sm >= 2.0 ? 48 : 96) * 1024;
             }
         }
     }
     const int64_t run = (chunks + best.cluster - 1) / best.cluster;
-    best.x_chunks = std::max<int64_t>(1, 16 * 1024 / x_chunk / best.ksplit) * best.ksplit;
+    best.x_chunks = std::max<int64_t>(1, best.x_bytes / x_chunk / best.ksplit) * best.ksplit;
     best.x_chunks = std::min<int64_t>(best.x_chunks, (run + best.ksplit - 1) / best.ksplit * best.ksplit);
     best.ring_bytes = std::max<size_t>(best.stages * record, kTokens * kPartStride * 4);
     best.ring_bytes = (best.ring_bytes + 127) / 128 * 128;
