@@ -85,8 +85,8 @@ struct RowShape {
     int per_cta;   // rows
 };
 
-// `most`: the most runs that a thread may hold.
-RowShape row_shape(int64_t width, int64_t rows, int sms, int most) {
+// `most`: the most runs that a thread may hold; `norm`: the norm, not the gate.
+RowShape row_shape(int64_t width, int64_t rows, int sms, int most, bool norm) {
     const int64_t runs = (width + 7) / 8;
     // Few rows: a thread per run, which spreads the row's latency over the CTA.
     // Many rows: two runs a thread and CTAs of at most 512 threads (2048 rows of
@@ -101,8 +101,8 @@ RowShape row_shape(int64_t width, int64_t rows, int sms, int most) {
         }
         for (held = 2; held < most && runs > static_cast<int64_t>(held) * 512;) held *= 2;
     }
-    while (held <= most && runs > static_cast<int64_t>(held) * mvq::max_row_threads(held)) held *= 2;
-    if (held > most) return {mvq::max_row_threads(0), 0, 1};
+    while (held <= most && runs > static_cast<int64_t>(held) * mvq::max_row_threads(held, norm)) held *= 2;
+    if (held > most) return {mvq::max_row_threads(0, norm), 0, 1};
     return {static_cast<int>(((runs + held - 1) / held + 31) / 32 * 32), held, 1};
 }
 
@@ -124,7 +124,7 @@ cudaError_t launch_row_held(const P& p, RowShape shape, int64_t rows, void* stre
 
 template <typename T, int OUT, template <typename, int, bool, int> class Kernel, typename P>
 cudaError_t launch_row_access(const P& p, bool runs, int64_t width, int64_t rows, int sms, void* stream) {
-    const RowShape shape = row_shape(width, rows, sms, runs ? 8 : 2);
+    const RowShape shape = row_shape(width, rows, sms, runs ? 8 : 2, Kernel<T, OUT, true, 1>::norm());
     return runs ? launch_row_held<T, OUT, true, Kernel>(p, shape, rows, stream)
                 : launch_row_held<T, OUT, false, Kernel>(p, shape, rows, stream);
 }
@@ -138,10 +138,12 @@ cudaError_t launch_row_type(const P& p, int64_t dtype, bool runs, int64_t width,
 
 template <typename T, int OUT, bool RUNS, int C>
 struct NormKernel {
+    static constexpr bool norm() { return true; }
     static auto get() { return mvq::add_rms_norm_kernel<T, OUT, RUNS, C>; }
 };
 template <typename T, int OUT, bool RUNS, int C>
 struct SiluKernel {
+    static constexpr bool norm() { return false; }
     static auto get() { return mvq::silu_mul_quant_kernel<T, OUT, RUNS, C>; }
 };
 

@@ -125,11 +125,7 @@ def _launch(entry, packed, index):
 
 
 def _add_rms_norm(x, residual, weight, eps, out, out_dtype, scales, residual_out):
-    if out is None and scales is None and residual_out is None and x.is_cuda:
-        found = _quant_native.binding().norm(x, residual, weight, eps, out_dtype)
-        if found is not None:
-            return found
-    # Not the usual call: everything is checked, and refused with its reason, here.
+    """What the binding's ``norm`` does, for every call: all is checked, and refused with its reason, here."""
     dtype, shape = x.dtype, x.shape
     code = DTYPE_CODES.get(dtype)
     _check(x.is_cuda and code is not None and shape, 'row operations take CUDA float tensors')
@@ -188,6 +184,10 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, 
     out may be x.
     """
     _check(residual is not None, 'add_rms_norm needs a residual')
+    if out is None and residual_out is None and x.is_cuda:
+        found = _quant_native.binding().norm(x, residual, weight, eps, x.dtype)
+        if found is not None:
+            return found[0], found[2]
     out, _, total = _add_rms_norm(x, residual, weight, eps, out, x.dtype, None, residual_out)
     return out, total
 
@@ -202,6 +202,10 @@ def add_rms_norm_quant(x: torch.Tensor, residual: torch.Tensor | None, weight: t
     infinity a NaN scale and zeros. residual None: s is x itself, which is not copied.
     """
     _check(quant_dtype in QUANT_CODES, 'quant_dtype must be int8 or float8_e4m3fn')
+    if out is None and scales is None and residual_out is None and x.is_cuda:
+        found = _quant_native.binding().norm(x, residual, weight, eps, quant_dtype)
+        if found is not None:
+            return found
     return _add_rms_norm(x, residual, weight, eps, out, quant_dtype, scales, residual_out)
 
 
