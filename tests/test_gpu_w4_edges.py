@@ -10,6 +10,7 @@ import subprocess
 import sys
 from pathlib import Path
 
+import numpy as np
 import pytest
 import torch
 
@@ -223,3 +224,64 @@ def test_calls_that_the_short_way_leaves_to_the_checked_one_agree_with_it(dtype)
     g = torch.ones(96, dtype=dtype, device='cuda')
     a, b = add_rms_norm(y, y, g, 1), add_rms_norm(y, y, g, 1.0)
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize('m', [4, 5, 6, 7, 8, 9])
+@pytest.mark.parametrize('k,n', [(2048, 128), (2176, 4160), (2176, 64)])
+def test_both_sides_of_the_rule_between_the_two_kernels(dtype, m, k, n):
+    from micro_vllm_b200.w4_linear import w4_linear
+    weight, w = make(n, k, 128, True, seed=53)
+    x, scale = activations(m, k, dtype, seed=54)
+    y = w4_linear(x.cuda(), weight, x_scale=None if scale is None else scale.cuda(), out_dtype=torch.float32)
+    assert_linear(y, x, scale, w, group=128)
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize('m', [17, 40, 100, 250])
+@pytest.mark.parametrize('k,n', [(2048, 64), (256, 19072), (1152, 9500)])
+def test_few_and_many_weight_rows_at_every_count_of_tokens(dtype, m, k, n):
+    """Few weight rows take narrow passes over many tokens, many weight rows wide ones."""
+    from micro_vllm_b200.w4_linear import w4_linear
+    weight, w = make(n, k, 64, False, seed=55)
+    x, scale = activations(m, k, dtype, seed=56)
+    y = w4_linear(x.cuda(), weight, x_scale=None if scale is None else scale.cuda(), out_dtype=torch.float32)
+    assert_linear(y, x, scale, w, group=64)
+
+
+@pytest.mark.parametrize('m', [9, 16, 33, 70, 128])
+@pytest.mark.parametrize('group', [32, 128])
+def test_e4m3_rows_over_long_columns_give_the_same_bits_each_time(m, group):
+    from micro_vllm_b200.w4_linear import w4_linear
+    weight, w = make(300, 8256, group, True, seed=57)
+    x, scale = activations(m, 8256, torch.float8_e4m3fn, seed=58)
+    args = dict(x_scale=scale.cuda(), out_dtype=torch.float32)
+    x_gpu = x.cuda()
+    y = w4_linear(x_gpu, weight, **args)
+    assert_linear(y, x, scale, w, group=group)
+    for _ in range(30):
+        again = w4_linear(x_gpu, weight, **args)
+        assert torch.equal(torch.nan_to_num(again, nan=0.5), torch.nan_to_num(y, nan=0.5))
+
+
+@pytest.mark.parametrize('rows', [1, 700])
+@pytest.mark.parametrize('width', [12344, 14336, 14344, 16384])
+def test_wide_rows_at_the_border_of_what_a_thread_holds(rows, width):
+    from micro_vllm_b200.row_ops import add_rms_norm_quant, silu_mul_quant
+    from tests.w4_reference import as64, assert_quantized
+    gen = torch.Generator().manual_seed(59)
+    x, r = (torch.randn((rows, width), generator=gen).to(torch.bfloat16) for _ in range(2))
+    weight = torch.randn(width, generator=gen).to(torch.bfloat16)
+    q, scales, total = add_rms_norm_quant(x.cuda(), r.cuda(), weight.cuda(), 1e-6)
+    s = (x.float() + r.float()).to(torch.bfloat16)
+    assert torch.equal(total.cpu(), s)
+    s64 = as64(s)
+    y = as64(weight) * s64 / ((s64 ** 2).mean(-1, keepdims=True) + 1e-6) ** 0.5
+    # The sum of squares: a tree of at most width / 32 additions a thread and ten more, each off by half of
+    # fp32's step, halved by the root; then a handful of roundings.
+    assert_quantized(q, scales, y, torch.int8, (width / 32 / 2 + 16) * 2.0 ** -24)
+    g = torch.cat([x, r], dim=-1)
+    q, scales = silu_mul_quant(g.cuda())
+    g64, u64 = as64(x), as64(r)
+    # The exponent's argument (up to 2^3) is off by 2^-24 of itself, exp and division by two units each.
+    assert_quantized(q, scales, g64 / (1 + np.exp(-g64)) * u64, torch.int8, 16 * 2.0 ** -23)
