@@ -173,30 +173,34 @@ __device__ __forceinline__ float2 block_sum_max(float sum, float top) {
     return all;
 }
 
-// What turns a row's values v (y = v * amax / top_v) into its 8-bit numbers: v
-// times `mul`, or, where top / top_v would overflow, v * 2^100 times `mul`. A
-// mul of zero: the row has no scale (zeros, or a NaN or an infinity among them).
+// What turns a row's values v (y = v * amax / top_v) into its 8-bit numbers: y /
+// scale = v * (top / top_v), the factor as the sum of two fp32 numbers. With it the
+// quotient is off by half of fp32's step, so that one that fp32 holds -- a tie
+// between two 8-bit numbers among them -- comes out as it is; one rounded factor put
+// one tie in 17 on the wrong side. `shift`: a power of two that v is multiplied by
+// first where the factor's parts would leave fp32's range. A factor of zero: the row
+// has no scale (zeros, or a NaN or an infinity among them).
 struct RowScale {
-    float scale, mul;
-    bool tiny;
+    float scale, mul, rest, shift;
 };
 template <int OUT>
 __device__ __forceinline__ RowScale row_scale(float amax, float top_v) {
     constexpr float kTop = OUT == kOutI8 ? 127.0f : 448.0f;
     RowScale s;
     s.scale = amax < INFINITY ? amax / kTop : __int_as_float(0x7fffffff);
-    s.tiny = top_v < 0x1p-100f;
-    s.mul = s.scale > 0.0f ? kTop / (s.tiny ? top_v * 0x1p+100f : top_v) : 0.0f;
+    s.shift = top_v < 0x1p-80f ? 0x1p+80f : top_v > 0x1p+80f ? 0x1p-80f : 1.0f;
+    top_v *= s.shift;
+    s.mul = s.scale > 0.0f ? kTop / top_v : 0.0f;
+    s.rest = s.scale > 0.0f ? fmaf(-s.mul, top_v, kTop) / top_v : 0.0f;
     return s;
 }
 __device__ __forceinline__ void apply_scale(const RowScale& s, float (&v)[8]) {
-    if (s.mul == 0.0f || s.tiny) {  // the same for the whole row
+    if (s.mul == 0.0f || s.shift != 1.0f) {  // the same for the whole row
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = s.mul == 0.0f ? 0.0f : v[i] * 0x1p+100f * s.mul;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] *= s.mul;
+        for (int i = 0; i < 8; ++i) v[i] = s.mul == 0.0f ? 0.0f : v[i] * s.shift;
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = fmaf(v[i], s.mul, v[i] * s.rest);
 }
 
 struct NormParams {
