@@ -108,7 +108,8 @@ def _disjoint(out, others, same=()):
     for other in others:
         if other is None or not storage_overlaps(out, other):
             continue
-        exact = any(other is t for t in same) and out.data_ptr() == other.data_ptr() and (
+        # Strides count elements: at another element size, rows of the same strides lie over other rows.
+        exact = any(other is t for t in same) and out.dtype is other.dtype and out.data_ptr() == other.data_ptr() and (
             out.stride() == other.stride() or out.numel() <= out.shape[-1])
         _check(exact, 'an output must be the input itself or share no memory with it')
 
