@@ -604,7 +604,25 @@ __global__ void __launch_bounds__(kThreads, 4) w4_linear_kernel(const LinearPara
 // 40.5). Bound by the output's bytes.
 // A code's distance from its zero point is exact in 16 bits, and its product
 // with a scale has at most 4 + 11 bits, so that a 16-bit product with a scale of
-// the output's type (`same`) rounds exactly as the fp32 product does.
+// the output's type (`same`) rounds exactly as the fp32 product does. The distance
+// is taken as it is: with the products' power of two (Act<kBF16>) a scale from
+// 2^117 on would have to become an infinity.
+struct DistanceBF16 {
+    __device__ __forceinline__ static uint32_t zero_low(int z) { return (0xc300u + z) * 0x10001u; }  // -(128 + z)
+    __device__ __forceinline__ static uint32_t zero_high(int z) { return zero_low(z); }
+    __device__ __forceinline__ static uint32_t distance(uint32_t w, uint32_t z) {
+        const uint32_t v = and_xor(w, 0x000f000fu, 0x43084308u);  // 128 + code
+        const __nv_bfloat162 d =
+            __hadd2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&z));
+        return *reinterpret_cast<const uint32_t*>(&d);
+    }
+    __device__ __forceinline__ static void weights(uint32_t w, uint32_t zl, uint32_t zh, uint32_t (&a)[4]) {
+        a[0] = distance(w, zl);
+        a[1] = distance(w >> 4, zh);
+        a[2] = distance(w >> 8, zl);
+        a[3] = distance(w >> 12, zh);
+    }
+};
 template <typename T>
 struct PairOf;
 template <>
@@ -614,7 +632,7 @@ struct PairOf<__half> {
 };
 template <>
 struct PairOf<__nv_bfloat16> {
-    using Kind = Act<kBF16>;
+    using Kind = DistanceBF16;
     using Pair = __nv_bfloat162;
 };
 template <>
@@ -628,7 +646,7 @@ w4_dequantize_kernel(const uint8_t* records, int64_t total, int chunks, int reco
                      int scale_bf16, int n, int k, T* out, int64_t out_stride, int runs) {
     using Kind = typename PairOf<T>::Kind;
     using Pair = typename PairOf<T>::Pair;
-    constexpr bool kBf16 = std::is_same<Kind, Act<kBF16>>::value;
+    constexpr bool kBf16 = std::is_same<Kind, DistanceBF16>::value;
     mv::wait_for_prior_grid();
     mv::allow_next_grid();
     const int64_t piece = static_cast<int64_t>(blockIdx.x) * kDequantizeWarps + (threadIdx.x >> 5);
@@ -681,10 +699,8 @@ w4_dequantize_kernel(const uint8_t* records, int64_t total, int chunks, int reco
                     float f[8];
                     uint32_t v[4];
                     if (same) {
-                        // Kind's power of two goes to the scale first, which is exact.
-                        const uint32_t up = kBf16 ? 0x45004500u : 0x3c003c00u;  // 2^11, 1
                         const uint32_t bits = __byte_perm(scales, 0, half ? 0x3232 : 0x1010);
-                        const Pair sc = __hmul2(*reinterpret_cast<const Pair*>(&bits), *reinterpret_cast<const Pair*>(&up));
+                        const Pair sc = *reinterpret_cast<const Pair*>(&bits);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             Pair d = *reinterpret_cast<const Pair*>(&a[i >> 1][half + 2 * (i & 1)]);
@@ -698,7 +714,7 @@ w4_dequantize_kernel(const uint8_t* records, int64_t total, int chunks, int reco
                         for (int i = 0; i < 4; ++i) {
                             const uint32_t pair = a[i >> 1][half + 2 * (i & 1)];
                             const float2 d = scale_pair(pair, kBf16);
-                            f[2 * i] = d.x * Kind::kScale * scale, f[2 * i + 1] = d.y * Kind::kScale * scale;
+                            f[2 * i] = d.x * scale, f[2 * i + 1] = d.y * scale;
                         }
                         if constexpr (sizeof(T) == 2) {
 #pragma unroll
