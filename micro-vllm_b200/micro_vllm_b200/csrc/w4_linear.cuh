@@ -662,9 +662,11 @@ w4_dequantize_kernel(const uint8_t* records, int64_t total, int chunks, int reco
     // Rows that are not aligned go out through shared memory, so that a warp
     // stores 32 columns of one row at a time.
     __shared__ T rows_out[sizeof(T) == 2 ? kDequantizeWarps : 1][sizeof(T) == 2 ? 64 * 34 : 1];
+    // Plain loads: the kernel before may have written the records while this one was launched, which the read-only
+    // path does not allow for.
     uint4 codes[2];
 #pragma unroll
-    for (int rp = 0; rp < 2; ++rp) codes[rp] = __ldg(reinterpret_cast<const uint4*>(rec) + (h * 2 + rp) * 32 + lane);
+    for (int rp = 0; rp < 2; ++rp) codes[rp] = reinterpret_cast<const uint4*>(rec)[(h * 2 + rp) * 32 + lane];
     {
         const int gi = h / group_runs;
         // 16 bits: two lanes trade words, so that each holds eight columns in a row,
@@ -681,9 +683,9 @@ w4_dequantize_kernel(const uint8_t* records, int64_t total, int chunks, int reco
                 if (t & 1) w.x = got0, w.z = got1;
                 else w.y = got0, w.w = got1;
             }
-            const uint2 s = __ldg(reinterpret_cast<const uint2*>(rec + kCodeBytes + gi * 128 + g * 16 + rp * 8));
+            const uint2 s = *reinterpret_cast<const uint2*>(rec + kCodeBytes + gi * 128 + g * 16 + rp * 8);
             uint32_t z = 0;
-            if (has_zeros) z = __ldg(reinterpret_cast<const uint32_t*>(rec + kCodeBytes + groups * 128 + gi * 64 + g * 8 + rp * 4));
+            if (has_zeros) z = *reinterpret_cast<const uint32_t*>(rec + kCodeBytes + groups * 128 + gi * 64 + g * 8 + rp * 4);
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
                 const uint32_t scales = q ? s.y : s.x;

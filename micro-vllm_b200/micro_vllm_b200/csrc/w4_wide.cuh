@@ -411,7 +411,7 @@ w4_wide_kernel(const LinearParams p, const __grid_constant__ CUtensorMap xmap) {
 #pragma unroll
             for (int gi = 0; gi < kGroups; ++gi)
                 if (i < n)
-                    w[gi] = __ldg(reinterpret_cast<const uint32_t*>(scale + static_cast<int64_t>(i) * kRecord + gi * 128));
+                    w[gi] = *reinterpret_cast<const uint32_t*>(scale + static_cast<int64_t>(i) * kRecord + gi * 128);
         };
         // X that TMA cannot copy as it is: these warps store it, element by element at
         // worst (rows off a 16-byte boundary). e4m3 numbers that become fp16 come by TMA

@@ -30,3 +30,25 @@ def test_dequantize_scales_of_every_size(dtype, scale_dtype, zeros, offset):
     assert torch.equal(got.cpu(), expected)
     if not offset:
         assert torch.equal(w4_dequantize(weight, dtype).cpu(), expected)
+
+
+@pytest.mark.parametrize('k', [2048, 2056])
+def test_dequantize_reads_what_the_call_before_wrote(k):
+    """Records rewritten between calls on one stream, with no wait of the host, by torch's copies and between this
+    library's own launches, which may start before the kernel ahead of them ends."""
+    from micro_vllm_b200.w4_linear import W4Weight, w4_dequantize, w4_linear
+    pairs = [make(2048, k, 64, True, seed=s) for s in (3, 4)]
+    a = pairs[0][0]
+    live = W4Weight(torch.empty_like(a.records), a.shape, a.group_size, a.has_zeros, a.scale_dtype)
+    expected = [torch.from_numpy(w).float().to(torch.bfloat16).cuda() for _, w in pairs]
+    out = torch.empty((2048, k), dtype=torch.bfloat16, device='cuda')
+    x = torch.ones((16, k), dtype=torch.bfloat16, device='cuda')
+    products = [w4_linear(x, weight) for weight, _ in pairs]
+    for turn in range(20):
+        live.records.copy_(pairs[turn % 2][0].records)
+        w4_dequantize(live, out=out)
+        assert torch.equal(out, expected[turn % 2])
+        assert torch.equal(w4_linear(x, live), products[turn % 2])
+        live.records.copy_(pairs[1 - turn % 2][0].records)
+        w4_linear(x, live)
+        assert torch.equal(w4_dequantize(live, torch.bfloat16), expected[1 - turn % 2])
