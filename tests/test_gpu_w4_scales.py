@@ -52,3 +52,26 @@ def test_dequantize_reads_what_the_call_before_wrote(k):
         live.records.copy_(pairs[1 - turn % 2][0].records)
         w4_linear(x, live)
         assert torch.equal(w4_dequantize(live, torch.bfloat16), expected[1 - turn % 2])
+
+
+@pytest.mark.parametrize('m', [1, 5, 20])
+def test_fp32_rows_are_multiplied_to_their_last_bits(m):
+    """One number of x per row and group: y is its product with a weight, over one group a sum of one term.
+
+    x is the exact sum of three bf16 numbers. Their products with a code's distance (at most 4 bits) are exact, three
+    are added (each addition off by at most 2^-23 of the largest), then scaled and joined by at most three more
+    roundings of 2^-24: below 2^-20 of the value. Without its third number x would be off by up to 2^-16."""
+    from micro_vllm_b200.w4_linear import w4_linear
+    n, k = 130, 512
+    weight, w = make(n, k, 64, False, seed=5)
+    gen = torch.Generator().manual_seed(6)
+    x = torch.zeros((m, k))
+    column = torch.randint(0, k, (m,), generator=gen)
+    # Mantissas whose last eight bits are all ones: what the first two bf16 numbers leave is nearly 2^-16.
+    bits = torch.randint(0, 1 << 15, (m,), generator=gen, dtype=torch.int32) << 8 | 0xff | 127 << 23
+    x[torch.arange(m), column] = bits.view(torch.float32)
+    y = as64(w4_linear(x.cuda(), weight))
+    expected = as64(x[torch.arange(m), column])[:, None] * w.T[column.numpy()]
+    assert (np.abs(y - expected) <= 2.0 ** -20 * np.abs(expected)).all()
+    two = as64((x[torch.arange(m), column].view(torch.int32) & -256).view(torch.float32))[:, None] * w.T[column.numpy()]
+    assert not (np.abs(two - expected) <= 2.0 ** -20 * np.abs(expected)).all()  # what the bound would catch
