@@ -660,8 +660,8 @@ w4_dequantize_kernel(const uint8_t* records, int64_t total, int chunks, int reco
     const int group_runs = group / 32, groups = kChunk / group;
     const bool same = sizeof(T) == 2 && (scale_bf16 != 0) == kBf16;
     // Rows that are not aligned go out through shared memory, so that a warp
-    // stores 32 columns of one row at a time.
-    __shared__ T rows_out[sizeof(T) == 2 ? kDequantizeWarps : 1][sizeof(T) == 2 ? 64 * 34 : 1];
+    // stores 32 columns of one row at a time; written as 32-bit words.
+    __shared__ __align__(16) T rows_out[sizeof(T) == 2 ? kDequantizeWarps : 1][sizeof(T) == 2 ? 64 * 34 : 1];
     // Plain loads: the kernel before may have written the records while this one was launched, which the read-only
     // path does not allow for.
     uint4 codes[2];
