@@ -85,9 +85,10 @@ struct RowShape {
     int per_cta;   // rows
 };
 
-// `most`: the most runs that a thread may hold; `norm`: the norm, not the gate.
-RowShape row_shape(int64_t width, int64_t rows, int sms, int most, bool norm) {
+// `vector`: rows that are read a run at a time; `norm`: the norm, not the gate.
+RowShape row_shape(int64_t width, int64_t rows, int sms, bool vector, bool norm) {
     const int64_t runs = (width + 7) / 8;
+    const int most = vector ? 8 : 2;  // runs that a thread may hold
     // Few rows: a thread per run, which spreads the row's latency over the CTA.
     // Many rows: two runs a thread and CTAs of at most 512 threads (2048 rows of
     // 14336: 33.6 us, with at most 256 threads 37.9, with up to 1024 62), or eight
@@ -95,14 +96,28 @@ RowShape row_shape(int64_t width, int64_t rows, int sms, int most, bool norm) {
     // of 896: 9.9 and 10.6).
     int held = 1;
     if (rows > 2 * static_cast<int64_t>(sms)) {
-        if (runs <= 128) {
+        if (runs <= 32 * (vector ? 4 : most)) {
             while (runs > 32 * held) held *= 2;
             return {32, held, 8};
         }
-        for (held = 2; held < most && runs > static_cast<int64_t>(held) * 512;) held *= 2;
+        if (vector || !norm) {
+            for (held = 2; held < most && runs > static_cast<int64_t>(held) * 512;) held *= 2;
+        } else {
+            // The norm by elements has registers for one run a thread: two spill (2000
+            // rows of 4001 in bf16: 33.0 us, two runs 36.4; of 8191, where one run would
+            // take 1024 threads: 74.7 and 70.6), and in 1024 threads are behind a row
+            // that is read twice (1000 rows of 12001: 66.8 and 40.8). A warp that reads
+            // a row twice is ahead of a CTA where there are enough of them (8000 rows
+            // of 1001: 25.6 and 29.5; 1000 rows: 7.7 and 6.2).
+            if (runs <= 128 && rows > 8 * static_cast<int64_t>(sms)) return {32, 0, 8};
+            held = runs <= 512 ? 1 : 2;
+        }
     }
-    while (held <= most && runs > static_cast<int64_t>(held) * mvq::max_row_threads(held, norm)) held *= 2;
-    if (held > most) return {mvq::max_row_threads(0, norm), 0, 1};
+    const auto threads = [&](int held) {
+        return !vector && norm && held == 2 ? 512 : mvq::max_row_threads(held, norm);
+    };
+    while (held <= most && runs > static_cast<int64_t>(held) * threads(held)) held *= 2;
+    if (held > most) return {threads(0), 0, 1};
     return {static_cast<int>(((runs + held - 1) / held + 31) / 32 * 32), held, 1};
 }
 
@@ -111,6 +126,7 @@ cudaError_t launch_row_held(const P& p, RowShape shape, int64_t rows, void* stre
     const dim3 grid(static_cast<unsigned>((rows + shape.per_cta - 1) / shape.per_cta));
     const dim3 block(shape.threads, shape.per_cta);
     switch (shape.held) {
+        case 0: return launch(Kernel<T, OUT, RUNS, 0>::get(), grid, block, 0, 1, stream, p);
         case 1: return launch(Kernel<T, OUT, RUNS, 1>::get(), grid, block, 0, 1, stream, p);
         case 2: return launch(Kernel<T, OUT, RUNS, 2>::get(), grid, block, 0, 1, stream, p);
         default: break;
@@ -119,12 +135,12 @@ cudaError_t launch_row_held(const P& p, RowShape shape, int64_t rows, void* stre
         if (shape.held == 4) return launch(Kernel<T, OUT, RUNS, 4>::get(), grid, block, 0, 1, stream, p);
         if (shape.held == 8) return launch(Kernel<T, OUT, RUNS, 8>::get(), grid, block, 0, 1, stream, p);
     }
-    return launch(Kernel<T, OUT, RUNS, 0>::get(), grid, block, 0, 1, stream, p);
+    return cudaErrorInvalidConfiguration;  // a shape that no kernel was made for
 }
 
 template <typename T, int OUT, template <typename, int, bool, int> class Kernel, typename P>
 cudaError_t launch_row_access(const P& p, bool runs, int64_t width, int64_t rows, int sms, void* stream) {
-    const RowShape shape = row_shape(width, rows, sms, runs ? 8 : 2, Kernel<T, OUT, true, 1>::norm());
+    const RowShape shape = row_shape(width, rows, sms, runs, Kernel<T, OUT, true, 1>::norm());
     return runs ? launch_row_held<T, OUT, true, Kernel>(p, shape, rows, stream)
                 : launch_row_held<T, OUT, false, Kernel>(p, shape, rows, stream);
 }
