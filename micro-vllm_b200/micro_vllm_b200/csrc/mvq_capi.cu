@@ -85,10 +85,10 @@ struct RowShape {
     int per_cta;   // rows
 };
 
-// `vector`: rows that are read a run at a time; `norm`: the norm, not the gate.
-RowShape row_shape(int64_t width, int64_t rows, int sms, bool vector, bool norm) {
+// `vector`: rows that are read a run at a time; `most`: the most runs that a thread may hold; `norm`: the norm, not
+// the gate.
+RowShape row_shape(int64_t width, int64_t rows, int sms, bool vector, int most, bool norm) {
     const int64_t runs = (width + 7) / 8;
-    const int most = vector ? 8 : 2;  // runs that a thread may hold
     // Few rows: a thread per run, which spreads the row's latency over the CTA.
     // Many rows: two runs a thread and CTAs of at most 512 threads (2048 rows of
     // 14336: 33.6 us, with at most 256 threads 37.9, with up to 1024 62), or eight
@@ -96,7 +96,7 @@ RowShape row_shape(int64_t width, int64_t rows, int sms, bool vector, bool norm)
     // of 896: 9.9 and 10.6).
     int held = 1;
     if (rows > 2 * static_cast<int64_t>(sms)) {
-        if (runs <= 32 * (vector ? 4 : most)) {
+        if (runs <= 32 * (most < 4 ? most : 4)) {
             while (runs > 32 * held) held *= 2;
             return {32, held, 8};
         }
@@ -131,16 +131,19 @@ cudaError_t launch_row_held(const P& p, RowShape shape, int64_t rows, void* stre
         case 2: return launch(Kernel<T, OUT, RUNS, 2>::get(), grid, block, 0, 1, stream, p);
         default: break;
     }
-    if constexpr (RUNS) {
+    if constexpr (Kernel<T, OUT, RUNS, 1>::most() >= 4)
         if (shape.held == 4) return launch(Kernel<T, OUT, RUNS, 4>::get(), grid, block, 0, 1, stream, p);
+    if constexpr (Kernel<T, OUT, RUNS, 1>::most() >= 8)
         if (shape.held == 8) return launch(Kernel<T, OUT, RUNS, 8>::get(), grid, block, 0, 1, stream, p);
-    }
     return cudaErrorInvalidConfiguration;  // a shape that no kernel was made for
 }
 
 template <typename T, int OUT, template <typename, int, bool, int> class Kernel, typename P>
 cudaError_t launch_row_access(const P& p, bool runs, int64_t width, int64_t rows, int sms, void* stream) {
-    const RowShape shape = row_shape(width, rows, sms, runs, Kernel<T, OUT, true, 1>::norm());
+    using Runs = Kernel<T, OUT, true, 1>;
+    using Elements = Kernel<T, OUT, false, 1>;
+    const RowShape shape =
+        row_shape(width, rows, sms, runs, runs ? Runs::most() : Elements::most(), Runs::norm());
     return runs ? launch_row_held<T, OUT, true, Kernel>(p, shape, rows, stream)
                 : launch_row_held<T, OUT, false, Kernel>(p, shape, rows, stream);
 }
@@ -155,11 +158,15 @@ cudaError_t launch_row_type(const P& p, int64_t dtype, bool runs, int64_t width,
 template <typename T, int OUT, bool RUNS, int C>
 struct NormKernel {
     static constexpr bool norm() { return true; }
+    // Eight runs of fp32 spill: a row that is read twice is ahead of them (1024 rows of 14344 to e4m3 43.4 us, held
+    // 57.9; in bf16 31.9 and 23.6).
+    static constexpr int most() { return !RUNS ? 2 : sizeof(T) == 4 ? 4 : 8; }
     static auto get() { return mvq::add_rms_norm_kernel<T, OUT, RUNS, C>; }
 };
 template <typename T, int OUT, bool RUNS, int C>
 struct SiluKernel {
     static constexpr bool norm() { return false; }
+    static constexpr int most() { return RUNS ? 8 : 2; }
     static auto get() { return mvq::silu_mul_quant_kernel<T, OUT, RUNS, C>; }
 };
 
