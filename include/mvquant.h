@@ -120,6 +120,13 @@ MVQ_API int mvq_silu_mul_quant(const MvqSiluArgs* args, void* stream);
 MVQ_API int mvq_device_status(int32_t device, uint32_t* status);
 MVQ_API int mvq_clear_device_status(int32_t device);
 
+/*
+ * Exercises that path, as mv_selftest_wait_timeout does for libmvdecode.so: one
+ * warp on `stream` waits, as the kernels do, on a barrier that nothing completes,
+ * for limit_ns (at most 100 ms), gives up, sets the bit and returns.
+ */
+MVQ_API int mvq_selftest_wait_timeout(uint64_t limit_ns, void* stream);
+
 MVQ_API int mvq_abi_version(void);
 
 /* Message for the last non-MVQ_OK status returned on this thread. */

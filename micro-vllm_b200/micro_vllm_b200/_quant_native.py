@@ -50,7 +50,7 @@ pack_silu = _packer(SILU_FIELDS)
 
 ENTRY_POINTS = ('mvq_w4_linear', 'mvq_w4_dequantize', 'mvq_add_rms_norm', 'mvq_silu_mul_quant')
 EXPORTED_SYMBOLS = ENTRY_POINTS + ('mvq_abi_version', 'mvq_last_error', 'mvq_device_status',
-                                   'mvq_clear_device_status')
+                                   'mvq_clear_device_status', 'mvq_selftest_wait_timeout')
 DEVICE_STATUS_WAIT_TIMEOUT = 1
 
 
@@ -69,6 +69,8 @@ def library() -> ctypes.CDLL:
     lib.mvq_device_status.restype = lib.mvq_clear_device_status.restype = ctypes.c_int
     lib.mvq_device_status.argtypes = [ctypes.c_int32, ctypes.POINTER(ctypes.c_uint32)]
     lib.mvq_clear_device_status.argtypes = [ctypes.c_int32]
+    lib.mvq_selftest_wait_timeout.restype = ctypes.c_int
+    lib.mvq_selftest_wait_timeout.argtypes = [ctypes.c_uint64, ctypes.c_void_p]
     lib.mvq_abi_version.restype = ctypes.c_int
     lib.mvq_last_error.restype = ctypes.c_char_p
     version = lib.mvq_abi_version()

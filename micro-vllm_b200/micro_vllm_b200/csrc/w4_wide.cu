@@ -230,4 +230,14 @@ int mvq_clear_device_status(int32_t device) try {
     return mvq::fail(MVQ_ERR_CUDA, "unexpected C++ exception");
 }
 
+int mvq_selftest_wait_timeout(uint64_t limit_ns, void* stream) try {
+    if (limit_ns == 0 || limit_ns > 100000000ull)
+        return mvq::fail(MVQ_ERR_INVALID_ARGUMENT, "limit_ns must be in (0, 100 ms]");
+    mvq::wait_timeout_selftest_kernel<<<1, 32, 0, static_cast<cudaStream_t>(stream)>>>(limit_ns);
+    const cudaError_t err = cudaGetLastError();
+    return err == cudaSuccess ? MVQ_OK : mvq::cuda_fail(err, "self-test kernel launch");
+} catch (...) {
+    return mvq::fail(MVQ_ERR_CUDA, "unexpected C++ exception");
+}
+
 }  // extern "C"

@@ -120,15 +120,25 @@ __device__ __forceinline__ bool wide_try(uint32_t bar, uint32_t parity) {
         : "memory");
     return done != 0;
 }
-__device__ __forceinline__ bool wide_wait(uint32_t bar, uint32_t parity) {
+__device__ __forceinline__ bool wide_wait_lane(uint32_t bar, uint32_t parity, unsigned long long limit_ns) {
     if (wide_try(bar, parity)) return true;
     const unsigned long long start = mv::global_timer_ns();
     while (true) {
 #pragma unroll 1
         for (int i = 0; i < 16; ++i)
             if (wide_try(bar, parity)) return true;
-        if (mv::global_timer_ns() - start > mv::kWaitLimitNs) return false;
+        if (mv::global_timer_ns() - start > limit_ns) return false;
     }
+}
+// A whole warp's wait. One that gives up sets `failed` and the device status.
+__device__ __forceinline__ bool wide_wait(uint64_t* bar, uint32_t parity, volatile int* failed,
+                                          unsigned long long limit_ns = mv::kWaitLimitNs) {
+    const bool ok = __all_sync(0xffffffffu, wide_wait_lane(mv::smem_addr(bar), parity, limit_ns));
+    if (!ok) {
+        *failed = 1;
+        if ((threadIdx.x & 31) == 0) atomicOr(&mv::g_device_status, mv::kStatusWaitTimeout);
+    }
+    return ok;
 }
 __device__ __forceinline__ void wide_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -260,14 +270,7 @@ w4_wide_kernel(const LinearParams p, const __grid_constant__ CUtensorMap xmap) {
     fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);  // the same in every lane, for the compiler too
     const uint32_t d_col = tmem + kAB * Shape::kACols;
-    const auto wait = [&](uint64_t* bar, int parity) {  // of a whole warp
-        const bool ok = __all_sync(0xffffffffu, wide_wait(mv::smem_addr(bar), parity & 1));
-        if (!ok) {
-            s_failed = 1;
-            if (lane == 0) atomicOr(&mv::g_device_status, mv::kStatusWaitTimeout);
-        }
-        return ok;
-    };
+    const auto wait = [&](uint64_t* bar, int parity) { return wide_wait(bar, parity & 1, &s_failed); };
 
     if (warp < 8) {
         const int g = lane >> 2;
@@ -575,6 +578,18 @@ w4_wide_kernel(const LinearParams p, const __grid_constant__ CUtensorMap xmap) {
         }
     }
     if (p.cluster > 1) cluster_barrier();  // no CTA leaves while another reads its shared memory
+}
+
+// The kernel's wait on a barrier that nothing completes, with a limit of its own.
+__global__ void wait_timeout_selftest_kernel(unsigned long long limit_ns) {
+    __shared__ __align__(8) uint64_t bar;
+    __shared__ volatile int failed;
+    if (threadIdx.x == 0) {
+        mv::mbar_init(mv::smem_addr(&bar), 1);
+        mv::fence_mbar_init();
+    }
+    __syncwarp();
+    wide_wait(&bar, 0, &failed, limit_ns);
 }
 
 }  // namespace mvq
