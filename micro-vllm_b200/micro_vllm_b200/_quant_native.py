@@ -16,7 +16,7 @@ import struct
 from functools import lru_cache
 from pathlib import Path
 
-from . import _native
+from . import _native, _tensors
 
 # MVQUANT_LIBRARY may name another build of the same library (e.g. a tuning variant).
 LIB_PATH = Path(os.environ.get('MVQUANT_LIBRARY', Path(__file__).resolve().parent / 'lib' / 'libmvquant.so'))
@@ -92,6 +92,14 @@ def binding():
     loader.exec_module(module)
     module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in ENTRY_POINTS))
     return module
+
+
+def refuse_transforms(*tensors) -> None:
+    """Raise where one of the tensors (or None) asks for what the kernels pass by (_tensors.refuse_transforms)."""
+    if binding().any_transformed(*tensors):
+        for t in tensors:
+            if t is not None:
+                _tensors.refuse_transforms(t, 'a tensor of this call')
 
 
 def check(status: int) -> None:

@@ -7,7 +7,9 @@
 #include <Python.h>
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -37,11 +39,20 @@ int code_of(at::ScalarType t) {
     }
 }
 
+// Inside a function transform, or with a tangent of forward-mode differentiation.
+bool transformed(const at::Tensor& t) {
+    return t.key_set().has_any(c10::DispatchKeySet({c10::DispatchKey::FuncTorchBatched,
+                                                    c10::DispatchKey::FuncTorchGradWrapper,
+                                                    c10::DispatchKey::Functionalize})) ||
+           (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined());
+}
+
 // A plain tensor of the device, or null.
 const at::Tensor* tensor_of(PyObject* o, int device) {
     if (!THPVariable_CheckExact(o)) return nullptr;
     const at::Tensor& t = THPVariable_Unpack(o);
-    if (!t.is_cuda() || t.layout() != at::kStrided || t.is_neg() || (t.requires_grad() && at::GradMode::is_enabled()))
+    if (!t.is_cuda() || t.layout() != at::kStrided || t.is_neg() || (t.requires_grad() && at::GradMode::is_enabled()) ||
+        transformed(t))
         return nullptr;
     return device < 0 || t.get_device() == device ? &t : nullptr;
 }
@@ -53,7 +64,10 @@ int64_t row_stride(const at::Tensor& t, int64_t width) {
     return t.stride(0);
 }
 
-bool current(int device) { return c10::cuda::current_device() == device; }
+// Device `device` is current, and no mode is on that means to see torch's calls.
+bool current(int device) {
+    return c10::cuda::current_device() == device && !c10::impl::TorchDispatchModeTLS::any_modes_set();
+}
 void* stream_of(int device) { return c10::cuda::getCurrentCUDAStream(device).stream(); }
 
 at::Tensor fresh(at::IntArrayRef shape, at::ScalarType type, const at::Device& device) {
@@ -239,6 +253,14 @@ PyObject* guarded(PyObject* self, PyObject* const* a, Py_ssize_t count) {
     END_HANDLE_TH_ERRORS
 }
 
+// any_transformed(tensors or None...): whether one is transformed, or a mode is on.
+PyObject* any_transformed(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    bool found = c10::impl::TorchDispatchModeTLS::any_modes_set();
+    for (Py_ssize_t i = 0; i < count && !found; ++i)
+        found = THPVariable_Check(a[i]) && transformed(THPVariable_Unpack(a[i]));
+    return PyBool_FromLong(found);
+}
+
 // bind(linear, dequantize, norm, silu): the loaded library's entry points, as addresses.
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t count) {
     if (count != 4) {
@@ -262,6 +284,7 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t count) {
 
 PyMethodDef g_methods[] = {MVQ_METHOD("linear", guarded<linear>), MVQ_METHOD("dequantize", guarded<dequantize>),
                            MVQ_METHOD("norm", guarded<norm>), MVQ_METHOD("silu", guarded<silu>),
+                           MVQ_METHOD("any_transformed", guarded<any_transformed>),
                            MVQ_METHOD("bind", bind), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_mvq_binding", nullptr, -1, g_methods};
 

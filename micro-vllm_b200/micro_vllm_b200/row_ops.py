@@ -127,6 +127,8 @@ def _launch(entry, packed, index):
 
 def _add_rms_norm(x, residual, weight, eps, out, out_dtype, scales, residual_out):
     """What the binding's ``norm`` does, for every call: all is checked, and refused with its reason, here."""
+    if x.is_cuda:
+        _quant_native.refuse_transforms(x, residual, weight, out, scales, residual_out)
     dtype, shape = x.dtype, x.shape
     code = DTYPE_CODES.get(dtype)
     _check(x.is_cuda and code is not None and shape, 'row operations take CUDA float tensors')
@@ -222,6 +224,8 @@ def silu_mul_quant(gate_up: torch.Tensor, *, quant_dtype: torch.dtype = torch.in
         found = _quant_native.binding().silu(gate_up, quant_dtype)
         if found is not None:
             return found
+    if gate_up.is_cuda:
+        _quant_native.refuse_transforms(gate_up, out, scales)
     dtype, shape = gate_up.dtype, gate_up.shape
     code = DTYPE_CODES.get(dtype)
     _check(gate_up.is_cuda and code is not None and shape, 'row operations take CUDA float tensors')

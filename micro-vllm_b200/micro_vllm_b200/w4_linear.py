@@ -206,6 +206,8 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, bias: torch.Tensor | None = Non
         if y is not None:
             return y
     # Not the usual call: everything is checked, and refused with its reason, here.
+    if x.is_cuda:
+        _native.refuse_transforms(x, bias, residual, x_scale, out)
     n, k = weight.shape
     x_dtype = x.dtype
     code = ACTIVATION_CODES.get(x_dtype)
@@ -288,6 +290,7 @@ def w4_dequantize(weight: W4Weight, dtype: torch.dtype | None = None, *,
         out = _native.binding().dequantize(weight.packed, weight.records, dtype)
         if out is not None:
             return out
+    _native.refuse_transforms(weight.records, out)
     code = FLOAT_CODES.get(dtype)
     _check(code is not None, 'dtype must be float32, float16 or bfloat16')
     if out is None:
