@@ -42,8 +42,18 @@ class W4Weight:
     __slots__ = ('records', 'shape', 'group_size', 'has_zeros', 'scale_dtype', 'index', 'fixed', 'packed')
 
     def __init__(self, records, shape, group_size, has_zeros, scale_dtype):
+        shape = torch.Size(shape)
+        _check(len(shape) == 2 and min(shape) > 0, 'shape must be two positive sizes')
+        _check(group_size in GROUP_SIZES, 'group_size must be 32, 64 or 128')
+        _check(scale_dtype in SCALE_CODES, 'scale_dtype must be float16 or bfloat16')
+        _check(records.dtype == torch.uint8 and records.is_contiguous(), 'records must be a contiguous uint8 tensor')
+        per_group = 2 * TILE_ROWS + (TILE_ROWS if has_zeros else 0)
+        record = TILE_ROWS * CHUNK // 2 + CHUNK // group_size * per_group
+        size = -(-shape[0] // TILE_ROWS) * -(-shape[1] // CHUNK) * record
+        # The kernels read what the shape says: fewer bytes would be read past their end.
+        _check(records.numel() == size, f'records of this weight take {size} bytes')
         self.records = records
-        self.shape = torch.Size(shape)
+        self.shape = shape
         self.group_size = group_size
         self.has_zeros = has_zeros
         self.scale_dtype = scale_dtype
