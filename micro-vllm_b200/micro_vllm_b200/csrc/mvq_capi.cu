@@ -227,14 +227,26 @@ int mvq_w4_linear(const MvqLinearArgs* a, void* stream) try {
                 a->x_stride_row < (int64_t(1) << 38);
     const int kind = a->x_dtype == MVQ_DTYPE_E4M3 ? mvq::kF16 : static_cast<int>(a->x_dtype);
     const int group = static_cast<int>(a->group);
-    // The mma.sync kernel for few rows, whose number depends on what staging x and
-    // joining sums cost beside the stream of the weights. Measured (us, wide and
-    // narrow): 896 x 1152 in bf16 at four rows 3.8 and 4.2, at five 3.8 and 5.4; 3584 x
-    // 3584 at four 6.5 and 6.2, at eight 6.3 and 8.8; 3584 x 28672 in bf16 at five 19.7 and
-    // 19.1, at eight 20.1 and 21.3, in int8 at eight 17.4 and 15.7; 14336 x 3584 in int8 at
-    // eight 14.3 and 13.3.
-    const bool small = p.chunks <= 16 || (kind != mvq::kI8 && p.tiles <= 64);
-    const int few = small ? 4 : kind == mvq::kI8 ? 8 : 6;
+    // The mma.sync kernel for few rows: how many depends on the stream of the weights
+    // beside what each row costs it, and for 8-bit rows on what the tcgen05 kernel's
+    // fixed part is. Measured in groups of 128 (us, tcgen05 and mma.sync):
+    //   16 bits   896 x 1152    three rows 4.4, 4.5     four 4.2, 4.8
+    //             3584 x 4608   three 7.5, 7.4          four 7.5, 8.0
+    //             14336 x 3584  four 15.0, 14.3         five 15.0, 15.3
+    //             3584 x 28672  seven 20.5, 20.3        eight 20.5, 21.8
+    //             8192 x 57344  eight 79, 68
+    //   int8      2048 x 2048   four 4.8, 4.8           five 4.8, 5.5
+    //             3584 x 4608   seven 7.2, 7.2          eight 7.3, 8.2
+    //             14336 x 3584  eight 14.8, 13.6
+    //   e4m3      2048 x 2048   four 6.5, 5.8           five 6.5, 7.2
+    //             3584 x 4608   seven 10.4, 9.6         eight 10.5, 10.6
+    //             14336 x 3584  eight 21.5, 20.0
+    const int64_t size_in_records = static_cast<int64_t>(p.chunks) * p.tiles;
+    const int few = size == 1 ? (size_in_records < 1800 ? 4 : size_in_records < 4096 ? 7 : 8)
+                              : (size_in_records < 4096    ? 3
+                                 : size_in_records < 8192  ? 4
+                                 : size_in_records < 32768 ? 7
+                                                           : 8);
     const int64_t out_size = dtype_size(a->out_dtype);
     for (int64_t m0 = 0; m0 < a->m; m0 += kLaunchRows) {
         p.m = static_cast<int>(a->m - m0 < kLaunchRows ? a->m - m0 : kLaunchRows);
