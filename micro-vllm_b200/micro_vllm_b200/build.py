@@ -5,9 +5,8 @@
 libmvdecode.so holds the decode path (include/mvdecode.h), libmvquant.so the
 operators with 4-bit weights and 8-bit rows (include/mvquant.h), _mvq_binding.so
 their common calls as Python functions (torch's C++ API, host code only). Both
-libraries link the
-CUDA runtime statically and the first resolves the driver's tensor-map encoder
-at run time, so they need only the NVIDIA driver next to them.
+libraries link the CUDA runtime statically and resolve the driver's tensor-map
+encoder at run time, so they need only the NVIDIA driver next to them.
 """
 import os
 import re

@@ -5,16 +5,21 @@
 // Mathematics. W[n, k] = (code - zero) * scale per row n and group of k. The
 // kernel never forms the scaled weight: within a group it sums x * (code -
 // zero) -- code - zero is a small integer, exact in bf16, fp16 and int8 -- and
-// then adds scale * sum to the row's fp32 accumulator. So the only rounding of
-// 16-bit activations' results is the last one.
+// then adds scale * sum to the row's fp32 accumulator. So products are exact and
+// weights are never rounded; what is rounded before the result are the fp32
+// additions (within a group, of scaled groups, of the columns' parts) and the
+// product with each group's scale.
 //
 // What bounds it: the codes are read once, half a byte per weight, and each
 // weight costs about 1.4 instructions to become a bf16 (shift, mask-xor,
 // subtract on pairs), 1.1 an fp16, 0.4 an int8, against about 2.8 issue slots
-// per weight at the copy bandwidth. The records hold the codes in the order of
-// the A operand of mma.sync (16 weight rows x 16 or 32 columns), so a lane's 16
-// bytes become four operand registers by masks and shifts alone, and both the
-// 16-bit and the 8-bit instruction read the same records.
+// per weight at the copy bandwidth. Yet no pipe is at its limit over a launch (one
+// row through 3584 -> 28672 in bf16: ALU 41 %, issue slots 47 %, DRAM 30 %): what
+// is left is the latency of the chain from a record's words over their conversion
+// to the multiplication, which three warps per scheduler do not hide. The records
+// hold the codes in the order of the A operand of mma.sync (16 weight rows x 16 or
+// 32 columns), so a lane's 16 bytes become four operand registers by masks and
+// shifts alone, and both the 16-bit and the 8-bit instruction read the same records.
 #pragma once
 
 #include <cuda_fp8.h>
@@ -55,7 +60,7 @@ struct LinearParams {
     int x_units;       // x's rows may be copied by TMA
     int cluster;       // CTAs that share a tile's columns, each with a run of chunks
     int ksplit;        // warps of a CTA that share a tile's columns: its kWarps / ksplit tiles
-    int stages;        // records in flight per warp
+    int stages;        // records in flight per warp: 2 or 3
     int x_chunks;      // chunks of x staged at a time (a multiple of ksplit)
     int ring_bytes;    // shared memory of a warp: its records, later its partial sums
     const void* bias;
@@ -433,8 +438,7 @@ __global__ void __launch_bounds__(kThreads, 4) w4_linear_kernel(const LinearPara
     const int last = min(mine, (from + p.x_chunks) / p.ksplit);
     for (int i = from / p.ksplit; i < last; ++i) {
         if (p.stages == 2) cp_async_wait<1>();
-        else if (p.stages == 3) cp_async_wait<2>();
-        else cp_async_wait<3>();
+        else cp_async_wait<2>();
         __syncwarp();
         const uint32_t rec = ring + drain * kRecord;
         drain = drain + 1 == p.stages ? 0 : drain + 1;

@@ -9,7 +9,7 @@
 // as the mma.sync kernel does, and tcgen05.st.16x256b (int8: 16x128b) puts a
 // lane's registers, rows g and g + 8 and columns 16 e + 4 t + s, in place without
 // passing shared memory. X lies in shared memory (K-major, 128-byte swizzle).
-// Each group's D is its own accumulation, in one of two TMEM buffers; four other
+// Each group's D is its own accumulation, in one of two to eight TMEM buffers; other
 // warps add it, scaled, to fp32 sums in registers, a thread per weight row.
 //
 // What bounds it: as in the mma.sync kernel the codes' conversion, about 22
