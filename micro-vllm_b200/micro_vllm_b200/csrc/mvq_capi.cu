@@ -228,25 +228,37 @@ int mvq_w4_linear(const MvqLinearArgs* a, void* stream) try {
     const int kind = a->x_dtype == MVQ_DTYPE_E4M3 ? mvq::kF16 : static_cast<int>(a->x_dtype);
     const int group = static_cast<int>(a->group);
     // The mma.sync kernel for few rows: how many depends on the stream of the weights
-    // beside what each row costs it, and for 8-bit rows on what the tcgen05 kernel's
-    // fixed part is. Measured in groups of 128 (us, tcgen05 and mma.sync):
-    //   16 bits   896 x 1152    three rows 4.4, 4.5     four 4.2, 4.8
-    //             3584 x 4608   three 7.5, 7.4          four 7.5, 8.0
-    //             14336 x 3584  four 15.0, 14.3         five 15.0, 15.3
-    //             3584 x 28672  seven 20.5, 20.3        eight 20.5, 21.8
-    //             8192 x 57344  eight 79, 68
-    //   int8      2048 x 2048   four 4.8, 4.8           five 4.8, 5.5
-    //             3584 x 4608   seven 7.2, 7.2          eight 7.3, 8.2
-    //             14336 x 3584  eight 14.8, 13.6
-    //   e4m3      2048 x 2048   four 6.5, 5.8           five 6.5, 7.2
-    //             3584 x 4608   seven 10.4, 9.6         eight 10.5, 10.6
-    //             14336 x 3584  eight 21.5, 20.0
-    const int64_t size_in_records = static_cast<int64_t>(p.chunks) * p.tiles;
-    const int few = size == 1 ? (size_in_records < 1800 ? 4 : size_in_records < 4096 ? 7 : 8)
-                              : (size_in_records < 4096    ? 3
-                                 : size_in_records < 8192  ? 4
-                                 : size_in_records < 32768 ? 7
-                                                           : 8);
+    // beside what each row costs it, on the tcgen05 kernel's fixed part, which is
+    // larger for e4m3 rows, and on the commit and the wait that each group costs that
+    // kernel. Measured (us, tcgen05 and mma.sync):
+    //   groups of 128, 16 bits  896 x 1152    three rows 4.4, 4.5   four 4.2, 4.8
+    //                           3584 x 4608   three 7.5, 7.4        four 7.5, 8.0
+    //                           14336 x 3584  four 15.0, 14.3       five 15.0, 15.3
+    //                           3584 x 28672  seven 20.5, 20.3      eight 20.5, 21.8
+    //                           8192 x 57344  eight 79, 68
+    //                   int8    2048 x 2048   four 4.8, 4.8         five 4.8, 5.5
+    //                           3584 x 4608   seven 7.2, 7.2        eight 7.3, 8.2
+    //                           14336 x 3584  eight 14.8, 13.6
+    //                   e4m3    2048 x 2048   four 6.5, 5.8         five 6.5, 7.2
+    //                           3584 x 4608   seven 10.4, 9.6       eight 10.5, 10.6
+    //                           14336 x 3584  eight 21.5, 20.0
+    //   groups of 64, 16 bits   1536 x 2048   four 5.2, 5.2         five 5.2, 5.8
+    //                           3584 x 4608   seven 9.3, 8.9        eight 9.2, 9.9
+    //                           3584 x 28672  eight 25.8, 23.0      nine 25.9, 36.1
+    //                   int8    3584 x 3584   seven 7.6, 7.5        eight 7.6, 8.6
+    //                           3584 x 4608   eight 9.5, 9.0        nine 9.4, 10.8
+    //   groups of 32, 16 bits   1536 x 2048   four 6.2, 5.5         five 6.2, 6.3
+    //                           3584 x 3584   eight 10.0, 9.6       nine 9.9, 11.4
+    //                           3584 x 28672  eight 37.7, 24.7      nine 37.7, 39.7
+    const int64_t held = static_cast<int64_t>(p.chunks) * p.tiles;  // records
+    const int few = held < 1000    ? (size == 1 || group < 128 ? 4 : 3)
+                    : group == 32  ? 8
+                    : group == 64  ? (held < 1800 ? (size == 1 ? 7 : 4) : size == 1 || held >= 8192 ? 8 : 7)
+                    : size == 1    ? (held < 1800 ? 4 : held < 4096 ? 7 : 8)
+                    : held < 4096  ? 3
+                    : held < 8192  ? 4
+                    : held < 32768 ? 7
+                                   : 8;
     const int64_t out_size = dtype_size(a->out_dtype);
     for (int64_t m0 = 0; m0 < a->m; m0 += kLaunchRows) {
         p.m = static_cast<int>(a->m - m0 < kLaunchRows ? a->m - m0 : kLaunchRows);
