@@ -92,9 +92,10 @@ MVQ_API int mvq_w4_dequantize(const MvqDequantizeArgs* args, void* stream);
  * For each row: s = to_dtype(x + residual), y = weight * s * rsqrt(mean(s^2) +
  * eps) in fp32. residual_out (if not NULL) gets s. residual NULL: s = x.
  * out_dtype == dtype: out gets y, rounded once. MVQ_DTYPE_I8 / MVQ_DTYPE_E4M3:
- * scales[row] = max|y| / top (top 127 / 448) and out = round(y / scale), zeros
- * where the scale is zero; a row with a NaN or an infinite y gets a NaN scale
- * and zeros. residual_out may be x or residual; in dtype, out may be x.
+ * scales[row] = max|y| / top (top 127 / 448) and out = round(y / scale), ties to
+ * even, zeros where the scale is zero; a row with a NaN or an infinite y gets a
+ * NaN scale and zeros. residual_out may be x or residual; in dtype, out may be x
+ * (an 8-bit out may not lie over an input).
  */
 typedef struct MvqNormArgs {
     const void* x; int64_t x_stride_row; const void* residual; int64_t residual_stride_row;
@@ -104,7 +105,10 @@ typedef struct MvqNormArgs {
 } MvqNormArgs;
 MVQ_API int mvq_add_rms_norm(const MvqNormArgs* args, void* stream);
 
-/* y = silu(g) * u in fp32 for rows [g | u] of 2 * width elements; out and scales as above (8 bits only). */
+/*
+ * y = silu(g) * u in fp32 for rows [g | u] of 2 * width elements (zero for g below
+ * -88.72, where exp(-g) passes fp32's range); out and scales as above (8 bits only).
+ */
 typedef struct MvqSiluArgs {
     const void* gate_up; int64_t stride_row; void* out; int64_t out_stride_row; void* scales;
     int64_t rows; int64_t width; int64_t dtype; int64_t out_dtype;

@@ -14,7 +14,7 @@
 // weight costs about 1.4 instructions to become a bf16 (shift, mask-xor,
 // subtract on pairs), 1.1 an fp16, 0.4 an int8, against about 2.8 issue slots
 // per weight at the copy bandwidth. Yet no pipe is at its limit over a launch (one
-// row through 3584 -> 28672 in bf16: ALU 41 %, issue slots 47 %, DRAM 30 %): what
+// row through 3584 -> 28672 in bf16: ALU 43 %, issue slots 48 %, DRAM 32 %): what
 // is left is the latency of the chain from a record's words over their conversion
 // to the multiplication, which three warps per scheduler do not hide. The records
 // hold the codes in the order of the A operand of mma.sync (16 weight rows x 16 or

@@ -201,8 +201,9 @@ def add_rms_norm_quant(x: torch.Tensor, residual: torch.Tensor | None, weight: t
     """``add_rms_norm`` with its norm y in 8 bits: (q, scales, s).
 
     scales [...] fp32 = max|y| / 127 (int8) or / 448 (float8_e4m3fn) over each row,
-    q = round(y / scale); a row of zeros has scale 0 and zeros, a row with a NaN or an
-    infinity a NaN scale and zeros. residual None: s is x itself, which is not copied.
+    q = round(y / scale), ties to even; a row of zeros has scale 0 and zeros, a row with a NaN
+    or an infinity a NaN scale and zeros. residual None: s is x itself, which is not copied.
+    out shares no memory with an input.
     """
     _check(quant_dtype in QUANT_CODES, 'quant_dtype must be int8 or float8_e4m3fn')
     if out is None and scales is None and residual_out is None and x.is_cuda:
@@ -216,7 +217,9 @@ def silu_mul_quant(gate_up: torch.Tensor, *, quant_dtype: torch.dtype = torch.in
                    scales: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """silu(g) * u in 8 bits, the last dimension split as [g | u]: (q, scales) as in ``add_rms_norm_quant``.
 
-    The product stays in fp32 until its one rounding (``silu_mul`` rounds each step).
+    The product stays in fp32 until its one rounding (``silu_mul`` rounds each step): off by a few
+    2^-24 of itself and, for gates below zero, by |g| 2^-24. Below -88.72, where fp32 does not hold
+    exp(-g), a value is zero.
     """
     out_code = QUANT_CODES.get(quant_dtype)
     _check(out_code is not None, 'quant_dtype must be int8 or float8_e4m3fn')
