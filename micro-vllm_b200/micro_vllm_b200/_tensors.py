@@ -33,11 +33,6 @@ def storage_overlaps(left: torch.Tensor, right: torch.Tensor) -> bool:
     return left_start - right_start < right_size
 
 
-_TRACING_MODES = tuple(torch._C._TorchDispatchModeKey.__members__.values())  # functional, proxy and fake tensors
-_modes_on = torch._C._len_torch_dispatch_stack
-_wrapped = torch._C._functorch.is_functorch_wrapped_tensor
-
-
 def refuse_transforms(t: torch.Tensor, name: str) -> None:
     """Raise where a call on t's memory would leave out what torch is to do with t.
 
@@ -46,7 +41,9 @@ def refuse_transforms(t: torch.Tensor, name: str) -> None:
     torch's calls or replaces tensors (make_fx, fake tensors): the kernels' launches
     pass all of these by.
     """
-    if _wrapped(t) or (_modes_on() and any(torch._C._get_dispatch_mode(mode) is not None for mode in _TRACING_MODES)):
+    modes = torch._C._TorchDispatchModeKey.__members__.values()  # of functional, proxy and fake tensors
+    if torch._C._functorch.is_functorch_wrapped_tensor(t) or any(
+            torch._C._get_dispatch_mode(mode) is not None for mode in modes):
         raise RuntimeError(f'{name}: this operator cannot be traced, faked or transformed')
     if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled() and \
             forward_ad.unpack_dual(t).tangent is not None:
